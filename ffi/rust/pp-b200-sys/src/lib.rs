@@ -35,6 +35,7 @@ pub const PP_DEV_OFFSET_RANGE: u32 = 0x2;
 pub const PP_DEV_LENGTH_RANGE: u32 = 0x4;
 pub const PP_DEV_WAIT_TIMEOUT: u32 = 0x8;
 pub const PP_DEV_POSITION_RANGE: u32 = 0x10;
+pub const PP_DEV_WINDOW_RANGE: u32 = 0x20;
 
 pub const PP_ATTN_PLAN_READY: u32 = 0x1;
 pub const PP_ATTN_PREFETCH_HISTORY: u32 = 0x2;
@@ -114,6 +115,34 @@ pub struct PpQkvRope {
     pub reserved: [u32; 2],
 }
 
+/// A batch of packed prompts (`include/pp_b200_prompt.h`): q `[q_tokens, heads,
+/// head_dim]`, k and v `[kv_tokens, kv_heads, head_dim]`, strides in elements.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct PpPrompt {
+    pub struct_size: u32,
+    pub sequences: u32,
+    pub heads: u32,
+    pub kv_heads: u32,
+    pub head_dim: u32,
+    pub dtype: i32,
+    pub q_tokens: u32,
+    pub kv_tokens: u32,
+    pub causal: u32,
+    pub softmax_scale: f32,
+    pub flags: u32,
+    pub max_ctas: u32,
+    pub q_token_stride: u64,
+    pub q_head_stride: u64,
+    pub k_token_stride: u64,
+    pub k_head_stride: u64,
+    pub v_token_stride: u64,
+    pub v_head_stride: u64,
+    pub q: *const c_void,
+    pub k: *const c_void,
+    pub v: *const c_void,
+}
+
 extern "C" {
     pub fn pp_b200_abi_version() -> u32;
     pub fn pp_b200_last_error() -> *const c_char;
@@ -170,6 +199,23 @@ extern "C" {
     pub fn pp_b200_renyi_sample(raw: *const f32, uniforms: *const f32, bounds: *const u32, out: *mut u32, batch: u32,
                                 choices: u32, guidance: u32, alpha: f32, cfg: f32, token_offset: u32,
                                 stream: *mut c_void) -> i32;
+    pub fn pp_b200_prompt_workspace_size(prompt: *const PpPrompt) -> usize;
+    pub fn pp_b200_plan_prompt(prompt: *const PpPrompt, q_starts: *const u32, kv_starts: *const u32,
+                               workspace: *mut c_void, workspace_bytes: usize, status: *mut u32,
+                               stream: *mut c_void) -> i32;
+    pub fn pp_b200_prompt_attention(prompt: *const PpPrompt, q_starts: *const u32, kv_starts: *const u32,
+                                    out: *mut c_void, workspace: *mut c_void, workspace_bytes: usize,
+                                    status: *mut u32, stream: *mut c_void) -> i32;
+    pub fn pp_b200_prompt_append(arena: *const PpKvArena, k: *const c_void, v: *const c_void, dtype: i32, tokens: u32,
+                                 k_token_stride: u64, k_head_stride: u64, v_token_stride: u64, v_head_stride: u64,
+                                 starts: *const u32, offsets: *const u32, status: *mut u32,
+                                 stream: *mut c_void) -> i32;
+    pub fn pp_b200_token_logprobs_workspace_size(rows: u32, choices: u32, top: u32) -> usize;
+    pub fn pp_b200_token_logprobs(logits: *const c_void, dtype: i32, rows: u32, choices: u32, row_stride: u64,
+                                  targets: *const i32, bounds: *const u32, top: u32, logprob: *mut f32,
+                                  entropy: *mut f32, rank: *mut u32, top_ids: *mut u32, top_logprobs: *mut f32,
+                                  workspace: *mut c_void, workspace_bytes: usize, status: *mut u32,
+                                  stream: *mut c_void) -> i32;
     pub fn pp_b200_prepare(device: i32) -> i32;
     pub fn pp_b200_prepare_optional(device: i32, fusion: u32, split_k: u32, model_dtype: i32, head_width: u32,
                                     ffn_hidden: u32) -> i32;

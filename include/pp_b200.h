@@ -33,6 +33,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "pp_b200_prompt.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -54,6 +56,7 @@ extern "C" {
 #define PP_DEV_LENGTH_RANGE 0x4u     /* attention length > capacity: row output is NaN */
 #define PP_DEV_WAIT_TIMEOUT 0x8u     /* a bounded pipeline wait gave up: output undefined */
 #define PP_DEV_POSITION_RANGE 0x10u  /* RoPE position >= max_context: row not written */
+#define PP_DEV_WINDOW_RANGE 0x20u    /* window of legal tokens outside the choices: row outputs are NaN */
 
 /* Geometry of a caller-owned int8 KV arena for one layer, in the reference's
  * batch-arena layout (app/src/model/cache.rs:301-478, int8_cache.rs:326-359):
@@ -248,6 +251,84 @@ int32_t pp_b200_plan_ragged_float(const PpFloatKv* kv, const PpAttnParams* param
 int32_t pp_b200_decode_attention_float(const PpFloatKv* kv, const PpAttnParams* params, const void* q,
                                        uint64_t q_row_stride, const uint32_t* lengths, void* out, void* workspace,
                                        size_t workspace_bytes, uint32_t* status, void* stream);
+
+/* ---- whole prompts: attention over packed sequences, append, scoring ----
+ *
+ * The reference prefills with ordinary attention over bf16 K/V
+ * (app/src/model/mod.rs:706-720) and appends the prompt through quantize +
+ * slice_set (app/src/model/int8_cache.rs:314-324, cache.rs:415-425).
+ *
+ * q_starts, kv_starts: device u32 [sequences + 1], the first token of each
+ * sequence and the end of the last (not decreasing, the last one at most
+ * q_tokens / kv_tokens).  kv_starts NULL: the same as q_starts.  A sequence
+ * of n query tokens and m keys sees, without `causal`, all m keys; with it,
+ * query i sees keys 0 .. m - n + i, so that keys beyond the queries are the
+ * tokens before this chunk.  A query that sees no key gives NaN, as length 0
+ * does in pp_b200_decode_attention.  Rows of q behind the last sequence leave
+ * their rows of `out` as they were.  Starts that decrease or pass the tensors'
+ * rows set PP_DEV_LENGTH_RANGE, and nothing is written. */
+
+/* Workspace bytes of pp_b200_plan_prompt / pp_b200_prompt_attention for this
+ * geometry (independent of the lengths on the device). */
+size_t pp_b200_prompt_workspace_size(const PpPrompt* prompt);
+
+/* The work list of these sequences: tiles of query rows, longest first, and
+ * cut along the keys where there are too few of them to fill the GPU.  Every
+ * layer of a step reuses it with PP_ATTN_PLAN_READY (same geometry, strides
+ * apart, and same lengths).  q, k and v may be NULL here.
+ * status (nullable): PP_DEV_LENGTH_RANGE. */
+int32_t pp_b200_plan_prompt(const PpPrompt* prompt, const uint32_t* q_starts, const uint32_t* kv_starts,
+                            void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
+
+/* Attention of every query token over its own sequence, scores, softmax and
+ * sums in f32.  out: [q_tokens, heads, head_dim] of the prompt's dtype, dense.
+ * status (nullable): PP_DEV_LENGTH_RANGE, PP_DEV_WAIT_TIMEOUT. */
+int32_t pp_b200_prompt_attention(const PpPrompt* prompt, const uint32_t* q_starts, const uint32_t* kv_starts,
+                                 void* out, void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
+
+/* Quantize-and-append of packed prompts: token starts[b] + i of branch b goes
+ * to slot offsets[b] + i of the branch's rows, with the arithmetic of
+ * pp_b200_quantize bit for bit.  k, v: f32/bf16 [tokens, heads, head_dim] of
+ * the arena's heads and head_dim, head_dim contiguous, token and head strides
+ * in elements.  starts: device u32 [rows/heads + 1] as q_starts above
+ * (starts that decrease or pass `tokens` set PP_DEV_LENGTH_RANGE, and nothing
+ * is written); offsets: device u32 [rows/heads].  A token whose slot is
+ * beyond the capacity is not written (PP_DEV_OFFSET_RANGE).
+ * status (nullable): those and PP_DEV_NONFINITE_INPUT. */
+int32_t pp_b200_prompt_append(const PpKvArena* arena, const void* k, const void* v, int32_t dtype, uint32_t tokens,
+                              uint64_t k_token_stride, uint64_t k_head_stride, uint64_t v_token_stride,
+                              uint64_t v_head_stride, const uint32_t* starts, const uint32_t* offsets,
+                              uint32_t* status, void* stream);
+
+/* Workspace bytes of pp_b200_token_logprobs (0 when it needs none). */
+size_t pp_b200_token_logprobs_workspace_size(uint32_t rows, uint32_t choices, uint32_t top);
+
+/* Log probabilities of given tokens with entropy and the best alternatives,
+ * over the head outputs the sampler reads.
+ *   logits    f32/bf16 [rows, choices], row stride row_stride elements
+ *   targets   i32 [rows], the given token (a column of its row)
+ *   bounds    NULL, or u32 [rows, 2] = (start, count) of the row's window of
+ *             legal columns, as in pp_b200_renyi_sample
+ *   logprob   f32 [rows]: x[target] - log(sum over the window of exp(x));
+ *             -inf for a target outside the window (-1: no target)
+ *   entropy   f32 [rows]: -sum p log p, in nats
+ *   rank      u32 [rows]: columns of the window ahead of the target in the
+ *             order (larger logit first, lower column first), 0 for the best;
+ *             the window's size for a target outside it
+ *   top_ids, top_logprobs  u32 / f32 [rows, top], the first `top` (0 .. 32) of
+ *             that order; 0xffffffff and -inf beyond the window and for
+ *             columns whose logit is -inf.  NULL with top 0.
+ * Sums are in f32, the closing logarithm in f64.  A NaN or +inf logit in the
+ * window makes the row's logprob, entropy and top_logprobs NaN, as log-softmax
+ * does; NaN logits come last in the order (after -inf, and in no list of
+ * alternatives).  An empty window gives NaN, no alternatives and rank 0; one
+ * outside the choices the same, and PP_DEV_WINDOW_RANGE.
+ * status (nullable): PP_DEV_WINDOW_RANGE. */
+int32_t pp_b200_token_logprobs(const void* logits, int32_t dtype, uint32_t rows, uint32_t choices,
+                               uint64_t row_stride, const int32_t* targets, const uint32_t* bounds, uint32_t top,
+                               float* logprob, float* entropy, uint32_t* rank, uint32_t* top_ids,
+                               float* top_logprobs, void* workspace, size_t workspace_bytes, uint32_t* status,
+                               void* stream);
 
 /* Diagnostic: runs one bounded wait on a barrier that nothing completes, with
  * the library's wait loop and a limit of limit_us microseconds (1..10^6), so a

@@ -24,6 +24,7 @@ DEV_OFFSET_RANGE = 0x2
 DEV_LENGTH_RANGE = 0x4
 DEV_WAIT_TIMEOUT = 0x8
 DEV_POSITION_RANGE = 0x10
+DEV_WINDOW_RANGE = 0x20
 
 ATTN_PLAN_READY = 0x1
 ATTN_PREFETCH_HISTORY = 0x2
@@ -57,6 +58,12 @@ EXPORTED = (
     "pp_b200_float_attention_workspace_size",
     "pp_b200_plan_ragged_float",
     "pp_b200_decode_attention_float",
+    "pp_b200_prompt_workspace_size",
+    "pp_b200_plan_prompt",
+    "pp_b200_prompt_attention",
+    "pp_b200_prompt_append",
+    "pp_b200_token_logprobs_workspace_size",
+    "pp_b200_token_logprobs",
     "pp_b200_prepare",
     "pp_b200_prepare_optional",
 )
@@ -117,6 +124,32 @@ class PpQkvRope(C.Structure):
     ]
 
 
+class PpPrompt(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("sequences", C.c_uint32),
+        ("heads", C.c_uint32),
+        ("kv_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("q_tokens", C.c_uint32),
+        ("kv_tokens", C.c_uint32),
+        ("causal", C.c_uint32),
+        ("softmax_scale", C.c_float),
+        ("flags", C.c_uint32),
+        ("max_ctas", C.c_uint32),
+        ("q_token_stride", C.c_uint64),
+        ("q_head_stride", C.c_uint64),
+        ("k_token_stride", C.c_uint64),
+        ("k_head_stride", C.c_uint64),
+        ("v_token_stride", C.c_uint64),
+        ("v_head_stride", C.c_uint64),
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+    ]
+
+
 class PreconditionError(ValueError):
     """Status 1: invalid geometry or argument; nothing was launched."""
 
@@ -164,6 +197,12 @@ def _load() -> C.CDLL:
         "pp_b200_float_attention_workspace_size": (sz, [P(PpFloatKv), P(PpAttnParams)]),
         "pp_b200_plan_ragged_float": (i32, [P(PpFloatKv), P(PpAttnParams), vp, vp, sz, vp]),
         "pp_b200_decode_attention_float": (i32, [P(PpFloatKv), P(PpAttnParams), vp, u64, vp, vp, vp, sz, vp, vp]),
+        "pp_b200_prompt_workspace_size": (sz, [P(PpPrompt)]),
+        "pp_b200_plan_prompt": (i32, [P(PpPrompt), vp, vp, vp, sz, vp, vp]),
+        "pp_b200_prompt_attention": (i32, [P(PpPrompt), vp, vp, vp, vp, sz, vp, vp]),
+        "pp_b200_prompt_append": (i32, [P(PpKvArena), vp, vp, i32, u32, u64, u64, u64, u64, vp, vp, vp, vp]),
+        "pp_b200_token_logprobs_workspace_size": (sz, [u32, u32, u32]),
+        "pp_b200_token_logprobs": (i32, [vp, i32, u32, u32, u64, vp, vp, u32, vp, vp, vp, vp, vp, vp, sz, vp, vp]),
         "pp_b200_prepare": (i32, [i32]),
         "pp_b200_prepare_optional": (i32, [i32, u32, u32, i32, u32, u32]),
     }

@@ -31,11 +31,16 @@ SOURCES = [
     ("csrc/kernels/decoder.cu", ["-fmad=false", "-prec-div=true", "-prec-sqrt=true"]),
     ("csrc/kernels/sampling.cu", ["-fmad=false", "-prec-div=true", "-prec-sqrt=true"]),
     ("csrc/kernels/lanes.cu", []),
+    ("csrc/kernels/prompt.cu", []),
+    ("csrc/kernels/prompt_append.cu", ["-fmad=false", "-prec-div=true", "-prec-sqrt=true"]),
+    ("csrc/kernels/logprobs.cu", []),
     ("csrc/host/abi.cpp", []),
+    ("csrc/host/prompt.cpp", []),
     ("csrc/host/sched.cpp", []),
     ("csrc/host/selfcheck.cpp", []),
 ]
-HEADERS = ["csrc/kernels/common.cuh", "csrc/kernels/quant_row.cuh", "csrc/kernels/lanes.cuh", "csrc/host/internal.h"]
+HEADERS = ["csrc/kernels/common.cuh", "csrc/kernels/quant_row.cuh", "csrc/kernels/lanes.cuh", "csrc/kernels/prompt.cuh",
+           "csrc/host/internal.h"]
 
 
 def nvcc() -> str:
@@ -50,7 +55,7 @@ def _mtime(path: str) -> float:
 
 
 def _newest_dep() -> float:
-    deps = [os.path.join(HERE, h) for h in HEADERS] + [os.path.join(ROOT, "include", "pp_b200.h")]
+    deps = [os.path.join(HERE, h) for h in HEADERS] + [os.path.join(ROOT, "include", h) for h in ("pp_b200.h", "pp_b200_prompt.h")]
     return max(_mtime(p) for p in deps)
 
 

@@ -77,6 +77,7 @@ int32_t device_info(DeviceInfo& out) {
                         "CUDA_ERROR_NO_BINARY_FOR_GPU: this library is built for sm_100a (B200); device is sm_%d%d",
                         d.major, minor);
         if ((e = pp::configure_attention_kernels(dev)) != cudaSuccess) return cuda_fail(e, "kernel configuration");
+        if ((e = pp::configure_prompt_kernels()) != cudaSuccess) return cuda_fail(e, "kernel configuration");
         if (!g_encode) {
             void* fn = nullptr;
             cudaDriverEntryPointQueryResult q{};
@@ -292,9 +293,49 @@ int32_t encode_float_map(CUtensorMap* map, const void* base, uint64_t row_stride
 }  // namespace
 
 namespace pp {
+int32_t check_arena(const PpKvArena* a, const char* what) { return ::check_arena(a, what); }
+
 int32_t fail_msg(int32_t status, const char* msg) {
     g_last_error = msg;
     return status;
+}
+
+int32_t fail_fmt(int32_t status, const char* fmt, ...) {
+    char buf[1024];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    g_last_error = buf;
+    return status;
+}
+
+int32_t cuda_status(cudaError_t e, const char* what) { return e == cudaSuccess ? PP_STATUS_OK : cuda_fail(e, what); }
+
+int32_t device_sms(uint32_t* num_sms) {
+    DeviceInfo d;
+    int32_t s = device_info(d);
+    if (s == PP_STATUS_OK) *num_sms = (uint32_t)d.num_sms;
+    return s;
+}
+
+// Row-major tiles with the 128-byte swizzle; dims[0] is the contiguous one and
+// strides (bytes) are those of dims 1 .. rank - 1.
+int32_t encode_tiled(CUtensorMap* map, CUtensorMapDataType type, uint32_t rank, const void* base, const uint64_t* dims,
+                     const uint64_t* strides, const uint32_t* box, const char* what) {
+    cuuint64_t d[5], st[4];
+    cuuint32_t b[5], es[5];
+    for (uint32_t i = 0; i < rank; ++i) {
+        d[i] = dims[i];
+        b[i] = box[i];
+        es[i] = 1;
+        if (i) st[i - 1] = strides[i - 1];
+    }
+    CUresult r = g_encode(map, type, rank, const_cast<void*>(base), d, st, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(PP_STATUS_PRECONDITION, "cuTensorMapEncodeTiled (%s) failed: %d", what, (int)r);
+    return PP_STATUS_OK;
 }
 
 int32_t current_context_id(unsigned long long* id) {
@@ -638,6 +679,7 @@ const char* pp_b200_status_message(uint32_t bits) {
     if (bits & PP_DEV_OFFSET_RANGE) return "batch KV needs context rebuild: append offset outside capacity";
     if (bits & PP_DEV_LENGTH_RANGE) return "INT8 attention lengths differ: length exceeds capacity (row output is NaN)";
     if (bits & PP_DEV_POSITION_RANGE) return "graph QKV/RoPE position exceeds the RoPE table (row not written)";
+    if (bits & PP_DEV_WINDOW_RANGE) return "token window outside the head's choices (row outputs are NaN)";
     return "unknown device status";
 }
 

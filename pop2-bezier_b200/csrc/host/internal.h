@@ -126,6 +126,119 @@ struct AttnLaunch {
     uint32_t ks_mis, vs_mis;  // element offset of the scale arrays inside their maps
 };
 
+// --------------------------------------------------- prompt attention plan
+//
+// Workspace layout (all offsets from the workspace base, 256-byte aligned):
+//   PromptHeader                            @ 0
+//   seq_base  u32 [sequences + 1]     first uncut entry of each sequence
+//   entries   PromptEntry [max_entries]     longest first
+//   counters  u32 [max_ctas * 4]      finished splits per cut item and 64 rows
+//                                     (zero between calls)
+//   acc       f32 [slots][slot_rows][head_dim]   partials of cut items
+//   ml        f32 [slots][slot_rows][2]          their maximum (log2 units), sum
+// An entry is cut only when its keys are more than its share of all the work,
+// (work in key tiles) / max_ctas, into ceil(keys / share) <= 2 keys / share
+// pieces: at most 2 max_ctas slots and max_ctas cut items, kv_heads included.
+struct PromptHeader {
+    uint32_t n_entries;
+    uint32_t n_items;  // entries * kv_heads
+    uint32_t next;     // next item to hand out beyond the grid's first ones (zero between calls)
+    uint32_t pad[5];
+};
+
+struct PromptEntry {
+    uint32_t q0, nq;              // first row of the sequence in q, its length
+    uint32_t k0, nk;              // the same of its keys
+    uint32_t tok0;                // first token of the entry, within the sequence
+    uint32_t kv_begin, kv_end;    // keys of this piece, within the sequence
+    uint32_t split, n_splits;     // which piece of how many
+    uint32_t slot0;               // slot of piece s and head h: (slot0 + s) * kv_heads + h
+    uint32_t counter;             // counters of head h: 4 * (counter * kv_heads + h)
+    uint32_t pad;
+};
+
+struct PromptWsLayout {
+    size_t seq_base, entries, counters, acc, ml, total;
+    uint32_t max_entries, max_slots, slot_rows, max_ctas;
+};
+
+inline PromptWsLayout prompt_ws_layout(uint32_t sequences, uint32_t q_tokens, uint32_t heads, uint32_t kv_heads,
+                                       uint32_t head_dim, uint32_t max_ctas) {
+    PromptWsLayout l{};
+    const uint32_t group = heads / kv_heads, per_entry = 2 * (128 / group);
+    l.max_ctas = max_ctas;
+    l.max_slots = 2 * max_ctas;
+    l.max_entries = q_tokens / per_entry + sequences + l.max_slots;
+    l.slot_rows = q_tokens <= 128 / group ? 128u : 256u;
+    size_t off = 256;
+    l.seq_base = off;
+    off = align_up(off + 4ull * (sequences + 1ull), 256);
+    l.entries = off;
+    off = align_up(off + sizeof(PromptEntry) * (size_t)l.max_entries, 256);
+    l.counters = off;
+    off = align_up(off + 16ull * max_ctas, 256);
+    l.acc = off;
+    off = align_up(off + 4ull * l.max_slots * l.slot_rows * head_dim, 256);
+    l.ml = off;
+    off = align_up(off + 8ull * l.max_slots * l.slot_rows, 256);
+    l.total = off;
+    return l;
+}
+
+struct PromptLaunch {
+    PpPrompt g;
+    const uint32_t* q_starts;
+    const uint32_t* kv_starts;
+    void* out;
+    unsigned char* ws;
+    PromptWsLayout layout;
+    uint32_t* status;
+    float scale_log2;
+    uint32_t num_sms;
+    bool vec;     // rows of q, k and v lie on 16-byte boundaries
+};
+
+cudaError_t configure_prompt_kernels();
+int32_t check_arena(const PpKvArena* a, const char* what);
+cudaError_t launch_prompt_plan(const PromptLaunch& L, cudaStream_t stream);
+cudaError_t launch_prompt_rows(const PromptLaunch& L, cudaStream_t stream);
+
+// Append of packed prompts: see prompt_append.cu.
+struct PromptAppendLaunch {
+    const PpKvArena* arena;
+    const void* k;
+    const void* v;
+    bool bf16;
+    uint32_t tokens;
+    uint64_t k_ts, k_hs, v_ts, v_hs;
+    const uint32_t* starts;
+    const uint32_t* offsets;
+    uint32_t* status;
+    bool vec;  // rows of k and v lie on 16-byte boundaries
+    uint32_t num_sms;
+};
+
+// Log probabilities of given tokens: see logprobs.cu.
+struct LogprobsLaunch {
+    const void* logits;
+    bool bf16;
+    uint32_t rows, choices, top;
+    uint64_t row_stride;
+    const int32_t* targets;
+    const uint32_t* bounds;
+    float* logprob;
+    float* entropy;
+    uint32_t* rank;
+    uint32_t* top_ids;
+    float* top_logprobs;
+    unsigned char* ws;
+    uint32_t* status;
+    uint32_t num_sms;
+};
+
+cudaError_t launch_prompt_append(const PromptAppendLaunch& P, cudaStream_t stream);
+cudaError_t launch_token_logprobs(const LogprobsLaunch& L, cudaStream_t stream);
+
 // QKV RoPE (+ int8 append): see decoder.cu.
 struct QkvRopeLaunch {
     const void* qkv;
@@ -168,6 +281,14 @@ uint32_t attention_float_stage_tokens(uint32_t head_dim, int kv_kind);
 cudaError_t launch_wait_probe(uint32_t* status, uint64_t limit_ns, cudaStream_t stream);
 cudaError_t launch_lane_uniforms(const uint64_t* seeds, uint64_t* draws, const uint32_t* active, uint32_t rows,
                                  float* out, cudaStream_t stream);
+
+// What the host files share (abi.cpp): the error string, the cached device
+// properties and the driver's tensor map encoder.
+int32_t fail_fmt(int32_t status, const char* fmt, ...);
+int32_t cuda_status(cudaError_t e, const char* what);
+int32_t device_sms(uint32_t* num_sms);
+int32_t encode_tiled(CUtensorMap* map, CUtensorMapDataType type, uint32_t rank, const void* base, const uint64_t* dims,
+                     const uint64_t* strides, const uint32_t* box, const char* what);
 
 // Records `msg` as the calling thread's last error and returns `status`.
 int32_t fail_msg(int32_t status, const char* msg);

@@ -1,0 +1,558 @@
+// Attention of whole prompts: the plan of a batch of packed sequences, and the
+// CUDA-core kernel that takes f32 tensors and rows off the 16-byte grid.
+#include <math_constants.h>
+
+#include "prompt.cuh"
+
+namespace pp {
+namespace {
+
+// ----------------------------------------------------------------- the plan
+//
+// One CTA.  Cuts every sequence into entries of 2 * tpt query tokens, counts
+// the key tiles each sees, and writes them longest first (64 classes of
+// length), because the attention CTAs take items in this order as they become
+// free: the last ones taken are the shortest.  Where the whole batch has fewer
+// key tiles than it takes to keep every CTA busy with whole entries, an entry
+// longer than its share is cut into equal pieces along the keys.
+constexpr int kPlanThreads = 1024;
+constexpr uint32_t kClasses = 64;
+#ifndef PP_PROMPT_MIN_SHARE
+#define PP_PROMPT_MIN_SHARE 2
+#endif
+
+struct PlanArgs {
+    const uint32_t* q_starts;
+    const uint32_t* kv_starts;
+    unsigned char* ws;
+    PromptWsLayout l;
+    uint32_t sequences, q_tokens, kv_tokens, causal, tpt, kv_heads;
+    uint32_t* status;
+};
+
+// Exclusive scan over the block; `total` gets the sum.
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* warp_tot, uint32_t& total) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    uint32_t inc = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+    }
+    __syncthreads();  // the totals of the scan before have been read
+    if (lane == 31) warp_tot[w] = inc;
+    __syncthreads();
+    if (w == 0) {
+        uint32_t t = lane < (int)(blockDim.x >> 5) ? warp_tot[lane] : 0u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, t, o);
+            if (lane >= o) t += y;
+        }
+        warp_tot[lane] = t;
+    }
+    __syncthreads();
+    total = warp_tot[31];
+    return inc - x + (w ? warp_tot[w - 1] : 0u);
+}
+
+// Entry `e` before cutting: its sequence and the number of key tiles it sees.
+__device__ __forceinline__ uint32_t entry_of(const PlanArgs& a, const uint32_t* seq_base, uint32_t e, PromptEntry& p) {
+    uint32_t lo = 0, hi = a.sequences;  // seq_base[lo] <= e < seq_base[hi]
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (seq_base[mid] <= e) lo = mid;
+        else hi = mid;
+    }
+    p.q0 = a.q_starts[lo];
+    p.nq = a.q_starts[lo + 1] - p.q0;
+    p.k0 = a.kv_starts[lo];
+    p.nk = a.kv_starts[lo + 1] - p.k0;
+    p.tok0 = (e - seq_base[lo]) * 2 * a.tpt;
+    p.kv_begin = 0;
+    p.kv_end = prompt_visible(p, min(p.nq, p.tok0 + 2 * a.tpt) - 1, a.causal);
+    return max(1u, (uint32_t)(((uint64_t)p.kv_end + kPromptKeyTile - 1) / kPromptKeyTile));
+}
+
+__global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArgs a) {
+    __shared__ uint32_t warp_tot[32], hist[kClasses], cursor[kClasses];
+    __shared__ uint32_t bad, longest, slots, cuts;
+    __shared__ unsigned long long work;
+    const uint32_t t = threadIdx.x;
+    PromptHeader* hdr = reinterpret_cast<PromptHeader*>(a.ws);
+    uint32_t* seq_base = reinterpret_cast<uint32_t*>(a.ws + a.l.seq_base);
+    PromptEntry* entries = reinterpret_cast<PromptEntry*>(a.ws + a.l.entries);
+    uint32_t* counters = reinterpret_cast<uint32_t*>(a.ws + a.l.counters);
+    if (t == 0) {
+        bad = longest = slots = cuts = 0;
+        work = 0;
+    }
+    if (t < kClasses) hist[t] = 0;
+    // launched as a programmatic dependent: the kernels before may still read
+    // the workspace or write the starts.  A dependent attention launch may
+    // start now; it waits for this kernel before it reads the plan.
+    pdl_wait_primary();
+    pdl_launch_dependents();
+    __syncthreads();
+    for (uint32_t i = t; i < 4 * a.l.max_ctas; i += kPlanThreads) counters[i] = 0;
+    for (uint32_t b = t; b < a.sequences; b += kPlanThreads) {
+        const uint32_t q0 = a.q_starts[b], q1 = a.q_starts[b + 1], k0 = a.kv_starts[b], k1 = a.kv_starts[b + 1];
+        if (q1 < q0 || q1 > a.q_tokens || k1 < k0 || k1 > a.kv_tokens) bad = 1;
+    }
+    __syncthreads();
+    uint32_t n = 0;
+    if (!bad) {
+        for (uint32_t b0 = 0; b0 < a.sequences; b0 += kPlanThreads) {
+            const uint32_t b = b0 + t;
+            const uint32_t nq = b < a.sequences ? a.q_starts[b + 1] - a.q_starts[b] : 0u;
+            uint32_t tot;
+            const uint32_t at = block_scan(nq / (2 * a.tpt) + (nq % (2 * a.tpt) != 0), warp_tot, tot);
+            if (b < a.sequences) seq_base[b] = n + at;
+            n += tot;
+        }
+    }
+    if (t == 0) {
+        seq_base[a.sequences] = n;
+        if (bad && a.status) atomicOr(a.status, PP_DEV_LENGTH_RANGE);
+    }
+    __syncthreads();
+    {
+        unsigned long long mine = 0;
+        uint32_t far = 0;
+        for (uint32_t e = t; e < n; e += kPlanThreads) {
+            PromptEntry p;
+            const uint32_t tiles = entry_of(a, seq_base, e, p);
+            mine += tiles;
+            far = max(far, tiles);
+        }
+        if (far) {
+            atomicAdd(&work, mine);
+            atomicMax(&longest, far);
+        }
+    }
+    __syncthreads();
+    const unsigned long long all = work * a.kv_heads;
+    const uint32_t share = (uint32_t)max((unsigned long long)PP_PROMPT_MIN_SHARE, (all + a.l.max_ctas - 1) / a.l.max_ctas);
+    const uint32_t most = min(longest, share);  // key tiles of the longest piece
+    for (uint32_t e = t; e < n; e += kPlanThreads) {
+        PromptEntry p;
+        const uint32_t tiles = entry_of(a, seq_base, e, p);
+        const uint32_t pieces = (tiles + share - 1) / share, len = (tiles + pieces - 1) / pieces;
+        atomicAdd(&hist[kClasses - 1 - (uint32_t)((uint64_t)(len - 1) * kClasses / most)], pieces);
+    }
+    __syncthreads();
+    if (t < 32) {
+        uint32_t lo = hist[2 * t], hi = hist[2 * t + 1], inc = lo + hi;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (t >= o) inc += y;
+        }
+        cursor[2 * t] = inc - lo - hi;
+        cursor[2 * t + 1] = inc - hi;
+        if (t == 31) {
+            hdr->n_entries = inc;
+            hdr->n_items = inc * a.kv_heads;
+            hdr->next = 0;
+        }
+    }
+    __syncthreads();
+    for (uint32_t e = t; e < n; e += kPlanThreads) {
+        PromptEntry p;
+        const uint32_t tiles = entry_of(a, seq_base, e, p);
+        const uint32_t pieces = (tiles + share - 1) / share, len = (tiles + pieces - 1) / pieces;
+        uint32_t at = atomicAdd(&cursor[kClasses - 1 - (uint32_t)((uint64_t)(len - 1) * kClasses / most)], pieces);
+        p.n_splits = pieces;
+        p.slot0 = p.counter = p.pad = 0;
+        if (pieces > 1) {
+            p.slot0 = atomicAdd(&slots, pieces);
+            p.counter = atomicAdd(&cuts, 1u);
+        }
+        const uint32_t end = p.kv_end;
+        for (uint32_t s = 0; s < pieces; ++s) {
+            // equal pieces of whole tiles: none is empty, as s * tiles / pieces is strictly increasing
+            p.split = s;
+            p.kv_begin = (uint32_t)((uint64_t)tiles * s / pieces) * kPromptKeyTile;
+            p.kv_end = s + 1 == pieces ? end : (uint32_t)((uint64_t)tiles * (s + 1) / pieces) * kPromptKeyTile;
+            entries[at + s] = p;
+        }
+    }
+}
+
+// ------------------------------------------------------ the CUDA-core kernel
+//
+// A work unit is 64 query rows of an item.  256 threads as 16 x 16: thread
+// (ty, tx) holds rows 4 ty .. 4 ty + 3; scores of keys tx + 16 j and channels
+// 4 tx + 64 h.  Online softmax in base 2 over key tiles of 64, all of it in
+// f32.  Products run two at a time on packed f32 pairs: pairs of channels for
+// q k', pairs of output channels for p v.
+constexpr int kRowsThreads = 256, kBN = 64;
+
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+template <bool BF>
+__device__ __forceinline__ float4 load4(const void* p, uint64_t i, bool vec) {
+    if constexpr (BF) {
+        const uint16_t* s = reinterpret_cast<const uint16_t*>(p) + i;
+        if (vec) {
+            const uint2 u = *reinterpret_cast<const uint2*>(s);
+            return make_float4(bf16_lo_to_f32(u.x), bf16_hi_to_f32(u.x), bf16_lo_to_f32(u.y), bf16_hi_to_f32(u.y));
+        }
+        return make_float4(bf16_lo_to_f32(s[0]), bf16_lo_to_f32(s[1]), bf16_lo_to_f32(s[2]), bf16_lo_to_f32(s[3]));
+    } else {
+        const float* s = reinterpret_cast<const float*>(p) + i;
+        if (vec) return *reinterpret_cast<const float4*>(s);
+        return make_float4(s[0], s[1], s[2], s[3]);
+    }
+}
+
+template <bool BF>
+__device__ __forceinline__ void store4(void* p, uint64_t i, float4 x) {
+    if constexpr (BF) {
+        uint2 u = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+        uint16_t* s = reinterpret_cast<uint16_t*>(p) + i;
+        *reinterpret_cast<uint2*>(s) = u;
+    } else {
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = x;
+    }
+}
+
+template <int D>
+struct RowsCfg {
+    static constexpr int LD = D + 4;  // rows 4 banks apart: 8 lanes' float4 cover all banks
+    static constexpr int SMEM = (2 * 64 * LD + 64 * D + 64 * (kBN + 4)) * 4;
+};
+
+template <int D, bool BF>
+__global__ void __launch_bounds__(kRowsThreads) prompt_rows_kernel(const PromptArgs a) {
+    using C = RowsCfg<D>;
+    constexpr int H = D / 64;  // channel groups of 4 a thread holds
+    extern __shared__ __align__(16) float sm[];
+    float* sq = sm;
+    float* sk = sq + 64 * C::LD;
+    float* sv = sk + 64 * C::LD;
+    float* sp = sv + 64 * D;
+    __shared__ uint32_t s_next, s_last;
+    const int t = threadIdx.x, tx = t & 15, ty = t >> 4;
+    PromptHeader* hdr = reinterpret_cast<PromptHeader*>(a.ws);
+    const PromptEntry* entries = reinterpret_cast<const PromptEntry*>(a.ws + a.l.entries);
+    float* acc_ws = reinterpret_cast<float*>(a.ws + a.l.acc);
+    float* ml_ws = reinterpret_cast<float*>(a.ws + a.l.ml);
+    uint32_t* counters = reinterpret_cast<uint32_t*>(a.ws + a.l.counters);
+    pdl_wait_primary();
+    const uint32_t units = hdr->n_items * 4, n_entries = hdr->n_entries;
+    uint32_t unit = blockIdx.x;
+    while (unit < units) {
+        const uint32_t item = unit >> 2, sub = unit & 3;
+        const uint32_t head = item / n_entries;
+        const PromptEntry e = entries[item - head * n_entries];
+        const uint32_t tile = sub >> 1, row0 = (sub & 1) * kPromptSubRows;
+        const uint32_t rows = min(a.tpt * a.group, row0 + kPromptSubRows);  // of the tile, up to this unit's end
+        const uint32_t tile_tok = e.tok0 + tile * a.tpt;
+        const bool any = row0 < rows && tile_tok + row0 / a.group < e.nq;
+        if (any) {
+            auto token_of = [&](uint32_t r) { return tile_tok + (row0 + r) / a.group; };
+            auto live = [&](uint32_t r) { return row0 + r < rows && token_of(r) < e.nq; };
+            // q, scaled so that scores are in log2 units
+            for (int i = t; i < 64 * (D / 4); i += kRowsThreads) {
+                const uint32_t r = i / (D / 4), c = i % (D / 4) * 4;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (live(r))
+                    x = load4<BF>(a.q, (uint64_t)(e.q0 + token_of(r)) * a.q_ts +
+                                           (uint64_t)(head * a.group + (row0 + r) % a.group) * a.q_hs + c, a.vec);
+                *reinterpret_cast<float4*>(sq + r * C::LD + c) = x;
+            }
+            uint32_t lim[4];  // keys that row 4 ty + i sees, within this piece
+            uint32_t last = 0, first = 0xffffffffu;
+            float m[4], z[4];
+            uint64_t acc[4][2 * H];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                lim[i] = live(4 * ty + i) ? min(e.kv_end, prompt_visible(e, token_of(4 * ty + i), a.causal)) : 0u;
+                m[i] = -CUDART_INF_F;
+                z[i] = 0.f;
+#pragma unroll
+                for (int j = 0; j < 2 * H; ++j) acc[i][j] = 0ull;
+            }
+            {  // keys that the unit's last row sees bound the loop; what its first row sees needs no mask
+                const uint32_t r_last = min(min(e.nq - tile_tok, a.tpt) * a.group, rows) - 1 - row0;
+                last = min(e.kv_end, prompt_visible(e, token_of(r_last), a.causal));
+                first = min(e.kv_end, prompt_visible(e, token_of(0), a.causal));
+            }
+            for (uint32_t n0 = e.kv_begin; n0 < last; n0 += kBN) {
+                __syncthreads();
+                for (int i = t; i < 64 * (D / 4); i += kRowsThreads) {
+                    const uint32_t r = i / (D / 4), c = i % (D / 4) * 4;
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+                    if (n0 + r < last) {
+                        const uint64_t row = (uint64_t)e.k0 + n0 + r;
+                        x = load4<BF>(a.k, row * a.k_ts + (uint64_t)head * a.k_hs + c, a.vec);
+                        y = load4<BF>(a.v, row * a.v_ts + (uint64_t)head * a.v_hs + c, a.vec);
+                    }
+                    *reinterpret_cast<float4*>(sk + r * C::LD + c) = x;
+                    *reinterpret_cast<float4*>(sv + r * D + c) = y;
+                }
+                __syncthreads();
+                uint64_t s2[4][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s2[i][j] = 0ull;
+#pragma unroll 4
+                for (int c = 0; c < D; c += 4) {
+                    ulonglong2 qv[4], kv[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        qv[i] = *reinterpret_cast<const ulonglong2*>(sq + (4 * ty + i) * C::LD + c);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        kv[j] = *reinterpret_cast<const ulonglong2*>(sk + (tx + 16 * j) * C::LD + c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            s2[i][j] = f2_fma(qv[i].y, kv[j].y, f2_fma(qv[i].x, kv[j].x, s2[i][j]));
+                }
+                const bool masked = n0 + kBN > first;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float s[4], top = -CUDART_INF_F;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float lo, hi;
+                        f2_unpack(s2[i][j], lo, hi);
+                        s[j] = (lo + hi) * a.scale_log2;
+                        if (n0 + tx + 16 * j >= lim[i]) s[j] = -CUDART_INF_F;
+                        top = fmaxf(top, s[j]);
+                    }
+#pragma unroll
+                    for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    const float mn = fmaxf(m[i], top);
+                    const float ref = mn == -CUDART_INF_F ? 0.f : mn;  // nothing seen yet: exp2(-inf) = 0
+                    const float f = exp2f(m[i] - ref);
+                    float sum = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float p = exp2f(s[j] - ref);
+                        sum += p;
+                        sp[(4 * ty + i) * (kBN + 4) + tx + 16 * j] = p;
+                    }
+#pragma unroll
+                    for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    z[i] = z[i] * f + sum;
+                    m[i] = mn;
+                    const uint64_t f2 = f2_pack(f, f);
+#pragma unroll
+                    for (int j = 0; j < 2 * H; ++j) acc[i][j] = f2_mul(acc[i][j], f2);
+                }
+                __syncwarp();  // the rows of a half-warp are its own
+                if (!masked) {
+#pragma unroll 4
+                    for (int n = 0; n < kBN; ++n) {
+                        ulonglong2 vv[H];
+#pragma unroll
+                        for (int h = 0; h < H; ++h)
+                            vv[h] = *reinterpret_cast<const ulonglong2*>(sv + n * D + 64 * h + 4 * tx);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float p = sp[(4 * ty + i) * (kBN + 4) + n];
+                            const uint64_t p2 = f2_pack(p, p);
+#pragma unroll
+                            for (int h = 0; h < H; ++h) {
+                                acc[i][2 * h] = f2_fma(p2, vv[h].x, acc[i][2 * h]);
+                                acc[i][2 * h + 1] = f2_fma(p2, vv[h].y, acc[i][2 * h + 1]);
+                            }
+                        }
+                    }
+                } else {
+                    // a key that a row does not see leaves it alone whatever its value holds (0 * NaN is NaN)
+                    const uint32_t end = min((uint32_t)kBN, last - n0);
+                    for (uint32_t n = 0; n < end; ++n) {
+                        ulonglong2 vv[H];
+#pragma unroll
+                        for (int h = 0; h < H; ++h)
+                            vv[h] = *reinterpret_cast<const ulonglong2*>(sv + n * D + 64 * h + 4 * tx);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (n0 + n >= lim[i]) continue;
+                            const float p = sp[(4 * ty + i) * (kBN + 4) + n];
+                            const uint64_t p2 = f2_pack(p, p);
+#pragma unroll
+                            for (int h = 0; h < H; ++h) {
+                                acc[i][2 * h] = f2_fma(p2, vv[h].x, acc[i][2 * h]);
+                                acc[i][2 * h + 1] = f2_fma(p2, vv[h].y, acc[i][2 * h + 1]);
+                            }
+                        }
+                    }
+                }
+            }
+            auto write_row = [&](int i, const float (&o)[4 * H], float sum) {
+                const uint32_t r = 4 * ty + i;
+                const uint64_t at = ((uint64_t)(e.q0 + token_of(r)) * a.heads + head * a.group + (row0 + r) % a.group) * D;
+#pragma unroll
+                for (int h = 0; h < H; ++h) {  // a row that sees no key: 0 / 0 = NaN
+                    store4<BF>(a.out, at + 64 * h + 4 * tx,
+                               make_float4(o[4 * h] / sum, o[4 * h + 1] / sum, o[4 * h + 2] / sum, o[4 * h + 3] / sum));
+                }
+            };
+            if (e.n_splits == 1) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (!live(4 * ty + i)) continue;
+                    float o[4 * H];
+#pragma unroll
+                    for (int j = 0; j < 2 * H; ++j) f2_unpack(acc[i][j], o[2 * j], o[2 * j + 1]);
+                    write_row(i, o, z[i]);
+                }
+            } else {
+                // partial of this piece; the CTA that brings the last one merges them in the order of the pieces
+                const uint32_t srow = tile * kPromptTileRows + row0;
+                auto slot_row = [&](uint32_t s, uint32_t r) {
+                    return (uint64_t)((e.slot0 + s) * a.kv_heads + head) * a.l.slot_rows + srow + r;
+                };
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (!live(4 * ty + i)) continue;
+                    const uint64_t at = slot_row(e.split, 4 * ty + i);
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+                        *reinterpret_cast<ulonglong2*>(acc_ws + at * D + 64 * h + 4 * tx) =
+                            make_ulonglong2(acc[i][2 * h], acc[i][2 * h + 1]);
+                    if (tx == 0) {
+                        ml_ws[2 * at] = m[i];
+                        ml_ws[2 * at + 1] = z[i];
+                    }
+                }
+                uint32_t* cnt = counters + 4 * (e.counter * a.kv_heads + head) + sub;
+                __threadfence();
+                __syncthreads();
+                if (t == 0) s_last = atomicAdd(cnt, 1u) + 1 == e.n_splits;
+                __syncthreads();
+                if (s_last) {
+                    __threadfence();
+                    if (t == 0) *cnt = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (!live(4 * ty + i)) continue;
+                        float top = -CUDART_INF_F, sum = 0.f, o[4 * H] = {};
+                        for (uint32_t s = 0; s < e.n_splits; ++s)
+                            top = fmaxf(top, __ldcg(ml_ws + 2 * slot_row(s, 4 * ty + i)));
+                        const float ref = top == -CUDART_INF_F ? 0.f : top;
+                        for (uint32_t s = 0; s < e.n_splits; ++s) {
+                            const uint64_t at = slot_row(s, 4 * ty + i);
+                            const float zs = __ldcg(ml_ws + 2 * at + 1), f = exp2f(__ldcg(ml_ws + 2 * at) - ref);
+                            if (zs == 0.f) continue;  // this row saw nothing of the piece
+                            sum += zs * f;
+#pragma unroll
+                            for (int h = 0; h < H; ++h) {
+                                const float4 x = __ldcg(reinterpret_cast<const float4*>(acc_ws + at * D + 64 * h + 4 * tx));
+                                o[4 * h] += x.x * f;
+                                o[4 * h + 1] += x.y * f;
+                                o[4 * h + 2] += x.z * f;
+                                o[4 * h + 3] += x.w * f;
+                            }
+                        }
+                        write_row(i, o, sum);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        if (t == 0) {
+            const uint32_t got = atomicAdd(&hdr->next, 1u);
+            if (got == units - 1) hdr->next = 0;  // every CTA has taken its last: ready for the next call
+            s_next = got + gridDim.x;
+        }
+        __syncthreads();
+        unit = s_next;
+    }
+}
+
+template <int D, bool BF>
+cudaError_t launch_rows(const PromptArgs& a, uint32_t ctas, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kRowsThreads);
+    cfg.dynamicSmemBytes = RowsCfg<D>::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, prompt_rows_kernel<D, BF>, a);
+}
+
+template <int D, bool BF>
+cudaError_t configure_rows() {
+    return cudaFuncSetAttribute(prompt_rows_kernel<D, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsCfg<D>::SMEM);
+}
+
+}  // namespace
+
+PromptArgs prompt_args(const PromptLaunch& L) {
+    PromptArgs a{};
+    a.q = L.g.q;
+    a.k = L.g.k;
+    a.v = L.g.v;
+    a.out = L.out;
+    a.ws = L.ws;
+    a.l = L.layout;
+    a.q_ts = L.g.q_token_stride;
+    a.q_hs = L.g.q_head_stride;
+    a.k_ts = L.g.k_token_stride;
+    a.k_hs = L.g.k_head_stride;
+    a.v_ts = L.g.v_token_stride;
+    a.v_hs = L.g.v_head_stride;
+    a.heads = L.g.heads;
+    a.kv_heads = L.g.kv_heads;
+    a.group = L.g.heads / L.g.kv_heads;
+    a.tpt = kPromptTileRows / a.group;
+    a.q_tokens = L.g.q_tokens;
+    a.kv_tokens = L.g.kv_tokens;
+    a.causal = L.g.causal;
+    a.scale_log2 = L.scale_log2;
+    a.vec = L.vec;
+    a.status = L.status;
+    return a;
+}
+
+cudaError_t configure_prompt_kernels() {
+    cudaError_t e;
+    if ((e = configure_rows<64, false>()) != cudaSuccess || (e = configure_rows<64, true>()) != cudaSuccess ||
+        (e = configure_rows<128, false>()) != cudaSuccess)
+        return e;
+    return configure_rows<128, true>();
+}
+
+cudaError_t launch_prompt_plan(const PromptLaunch& L, cudaStream_t stream) {
+    PlanArgs a{};
+    a.q_starts = L.q_starts;
+    a.kv_starts = L.kv_starts;
+    a.ws = L.ws;
+    a.l = L.layout;
+    a.sequences = L.g.sequences;
+    a.q_tokens = L.g.q_tokens;
+    a.kv_tokens = L.g.kv_tokens;
+    a.causal = L.g.causal;
+    a.tpt = kPromptTileRows / (L.g.heads / L.g.kv_heads);
+    a.kv_heads = L.g.kv_heads;
+    a.status = L.status;
+    return launch_pdl(prompt_plan_kernel, dim3(1), dim3(kPlanThreads), stream, a);
+}
+
+cudaError_t launch_prompt_rows(const PromptLaunch& L, cudaStream_t stream) {
+    const PromptArgs a = prompt_args(L);
+    const bool bf = L.g.dtype == PP_DTYPE_BF16;
+    // resident CTAs an SM by shared memory: 3 at head_dim 64, 1 at 128
+    if (L.g.head_dim == 64)
+        return bf ? launch_rows<64, true>(a, 3 * L.layout.max_ctas, stream)
+                  : launch_rows<64, false>(a, 3 * L.layout.max_ctas, stream);
+    return bf ? launch_rows<128, true>(a, L.layout.max_ctas, stream) : launch_rows<128, false>(a, L.layout.max_ctas, stream);
+}
+
+}  // namespace pp

@@ -14,6 +14,10 @@ Differences, all documented at the call:
   * split_tokens == 0 selects the balanced stream-K plan instead of one CTA
     per row; a non-zero split_tokens is clamped to [32, 1024] as the
     reference does.  Results agree within f32 reassociation for any split.
+
+prompt_attention is the prefill side: every token of a batch of packed prompts
+attends to its own sequence (the reference's ordinary causal attention,
+app/src/model/mod.rs:716-720, with K/V shared by groups of query heads).
 """
 from __future__ import annotations
 
@@ -113,3 +117,105 @@ def prepare_optional_kernels(device: torch.device | int, fusion: bool, split_k: 
     code = N.DTYPE_F32 if dtype == torch.float32 else N.DTYPE_BF16
     N.check(N.lib.pp_b200_prepare_optional(0 if idx is None else idx, int(fusion), int(split_k), code, head_width,
                                            ffn_hidden))
+
+
+_MSG_PROMPT = ("prompt attention requires CUDA BF16/F32 q [tokens,heads,64|128] and k, v [tokens,kv_heads,64|128] of one "
+               "type and device, heads a multiple (1..64) of kv_heads, head_dim contiguous")
+_MSG_STARTS = "prompt starts must be contiguous same-device U32 [sequences + 1]"
+
+
+def _starts(t: torch.Tensor, n: int | None, device: torch.device) -> int:
+    if t.dim() != 1 or t.numel() < 2 or (n is not None and t.numel() != n + 1) \
+            or t.dtype not in (torch.int32, torch.uint32) or not t.is_contiguous() or t.device != device:
+        raise N.PreconditionError(_MSG_STARTS)
+    return t.numel() - 1
+
+
+def prompt_struct(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sequences: int, *, causal: bool = True,
+                  softmax_scale: float = 0.0, plan_ready: bool = False, max_ctas: int = 0) -> N.PpPrompt:
+    """The C ABI's geometry of packed prompts, after its checks."""
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
+        raise N.PreconditionError(_MSG_PROMPT)
+    tokens, heads, d = q.shape
+    kv_tokens, kv_heads, kd = k.shape
+    dt = q.dtype
+    if not q.is_cuda or k.device != q.device or v.device != q.device or kd != d or d not in (64, 128) \
+            or dt not in (torch.float32, torch.bfloat16) or k.dtype != dt or v.dtype != dt or heads == 0 or kv_heads == 0 \
+            or heads % kv_heads or heads > 64 * kv_heads or q.stride(2) != 1 or k.stride(2) != 1 or v.stride(2) != 1:
+        raise N.PreconditionError(_MSG_PROMPT)
+    return N.PpPrompt(C.sizeof(N.PpPrompt), sequences, heads, kv_heads, d,
+                      N.DTYPE_F32 if dt == torch.float32 else N.DTYPE_BF16, tokens, kv_tokens, int(bool(causal)),
+                      softmax_scale, N.ATTN_PLAN_READY if plan_ready else 0, max_ctas, q.stride(0), q.stride(1),
+                      k.stride(0), k.stride(1), v.stride(0), v.stride(1), q.data_ptr(), k.data_ptr(), v.data_ptr())
+
+
+def prompt_workspace(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sequences: int, *, max_ctas: int = 0
+                     ) -> torch.Tensor:
+    """A workspace for plan_prompt / prompt_attention over tensors of these
+    shapes and that many sequences.  Calls that may run at the same time need
+    one each."""
+    g = prompt_struct(q, k, v, sequences, max_ctas=max_ctas)
+    with torch.cuda.device(q.device):
+        return torch.empty(int(N.lib.pp_b200_prompt_workspace_size(C.byref(g))), dtype=torch.uint8, device=q.device)
+
+
+def plan_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts: torch.Tensor, workspace: torch.Tensor, *,
+                kv_starts: torch.Tensor | None = None, causal: bool = True, max_ctas: int = 0,
+                status: torch.Tensor | None = None) -> None:
+    """Writes the work list of these sequences into `workspace`, for the
+    prompt_attention calls with plan_ready=True that follow: every layer of a
+    prefill has the same shapes and lengths."""
+    n = _starts(q_starts, None, q.device)
+    if kv_starts is not None:
+        _starts(kv_starts, n, q.device)
+    g = prompt_struct(q, k, v, n, causal=causal, max_ctas=max_ctas)
+    _prompt_buffers(q, workspace, status)
+    with torch.cuda.device(q.device):
+        N.check(N.lib.pp_b200_plan_prompt(C.byref(g), q_starts.data_ptr(), ops._ptr(kv_starts), workspace.data_ptr(),
+                                          workspace.numel(), ops._ptr(status), ops._stream(q)))
+
+
+def _prompt_buffers(q: torch.Tensor, workspace: torch.Tensor | None, status: torch.Tensor | None) -> None:
+    if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous()
+                                  or workspace.device != q.device):
+        raise N.PreconditionError("prompt workspace must be a contiguous same-device byte tensor")
+    if status is not None and (status.dtype not in (torch.int32, torch.uint32) or status.numel() < 1
+                               or status.device != q.device):
+        raise N.PreconditionError("prompt status must be a same-device U32 word")
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts: torch.Tensor, *,
+                     kv_starts: torch.Tensor | None = None, causal: bool = True, softmax_scale: float = 0.0,
+                     workspace: torch.Tensor | None = None, plan_ready: bool = False, max_ctas: int = 0,
+                     status: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of packed prompts; returns [tokens, heads, head_dim] of q's type.
+
+    q [tokens, heads, d], k and v [kv_tokens, kv_heads, d], bf16 or f32, any
+    token and head strides; q_starts int32/uint32 [sequences + 1] on the
+    device: sequence s holds the query tokens q_starts[s] .. q_starts[s + 1].
+    kv_starts does the same for the keys (default: the same tokens).  A causal
+    query i of n, with m keys, sees keys 0 .. m - n + i: with more keys than
+    queries it continues a sequence whose first m - n tokens came before (a
+    later chunk of a prompt, or a single token).  A query that sees no key
+    gives NaN; rows of `out` that no sequence holds are left as they were.
+    softmax_scale 0: 0.125 at d = 64, 1/sqrt(d) otherwise.  A status word gets
+    DEV_LENGTH_RANGE when the starts decrease or pass the tensors' ends (then
+    nothing is written)."""
+    n = _starts(q_starts, None, q.device)
+    if kv_starts is not None:
+        _starts(kv_starts, n, q.device)
+    g = prompt_struct(q, k, v, n, causal=causal, softmax_scale=softmax_scale, plan_ready=plan_ready, max_ctas=max_ctas)
+    _prompt_buffers(q, workspace, status)
+    if plan_ready and workspace is None:
+        raise N.PreconditionError("plan_ready needs the workspace that plan_prompt wrote")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        raise N.PreconditionError("prompt attention writes a dense [tokens,heads,head_dim] of q's type and device")
+    with torch.cuda.device(q.device):
+        if workspace is None:
+            workspace = torch.empty(N.lib.pp_b200_prompt_workspace_size(C.byref(g)), dtype=torch.uint8, device=q.device)
+        N.check(N.lib.pp_b200_prompt_attention(C.byref(g), q_starts.data_ptr(), ops._ptr(kv_starts), out.data_ptr(),
+                                               workspace.data_ptr(), workspace.numel(), ops._ptr(status),
+                                               ops._stream(q)))
+    return out

@@ -125,6 +125,30 @@ class Int8KvArena:
         N.check(N.lib.pp_b200_quant_append(C.byref(a), ops._ptr(k_new), ops._ptr(v_new), code, ops._ptr(offsets),
                                            int(commit), ops._ptr(status), ops._stream(k_new)))
 
+    def append_prompt(self, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, offsets: torch.Tensor, *,
+                      status: torch.Tensor | None = None) -> None:
+        """Quantize-and-append of packed prompts: k, v F32/BF16 [tokens, heads,
+        d] (any token and head strides); tokens starts[b] .. starts[b + 1] go
+        to the slots of branch b from offsets[b] on.  Codes and scales are
+        those of `append`, bit for bit.  A token whose slot is beyond the
+        capacity is not written (DEV_OFFSET_RANGE in the status word); starts
+        that decrease or pass the tokens write nothing (DEV_LENGTH_RANGE)."""
+        ops._require_cuda(k, v, starts, offsets, self.k, status)
+        if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or tuple(k.shape[1:]) != (self.heads, self.head_dim) \
+                or k.stride(2) != 1 or v.stride(2) != 1:
+            raise N.PreconditionError("INT8 prompt append requires F32/BF16 [tokens,heads,head_dim] of the arena's heads")
+        if starts.numel() != self.branches + 1 or offsets.numel() != self.branches:
+            raise N.PreconditionError("prompt starts and offsets and branch counts differ")
+        for t in (starts, offsets):
+            if t.dtype not in (torch.int32, torch.uint32) or not t.is_contiguous():
+                raise N.PreconditionError("prompt starts and offsets must be contiguous U32")
+        code = ops._dtype_code(k, "K/V input")
+        a = self.struct()
+        with torch.cuda.device(k.device):
+            N.check(N.lib.pp_b200_prompt_append(C.byref(a), k.data_ptr(), v.data_ptr(), code, k.shape[0], k.stride(0),
+                                                k.stride(1), v.stride(0), v.stride(1), starts.data_ptr(),
+                                                offsets.data_ptr(), ops._ptr(status), ops._stream(k)))
+
     def attention(self, q: torch.Tensor, lengths: torch.Tensor, **kw) -> torch.Tensor:
         """History-mode decode attention over this arena (see int8_kv_ops.decode_attention)."""
         return ops.decode_attention(q, self.k, self.v, self.k_scale, self.v_scale, lengths, self.heads, **kw)

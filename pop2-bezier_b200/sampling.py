@@ -1,11 +1,17 @@
-"""Device sampling after the output heads, on the C ABI.
+"""Device sampling and scoring after the output heads, on the C ABI.
 
 renyi_sample mirrors fused_sampling::sample (app/src/inference/
 fused_sampling.rs:69-90): Rényi-entropy truncated sampling with classifier-
 free guidance, one logical row per block, bit-identical to the reference's
 pp_renyi_sample.
+
+token_logprobs scores given tokens under the same heads: log probability,
+rank, entropy of the row and its best alternatives, as teacher-forced
+comparisons of two models read them (app/src/bin/kv_int8_acceptance.rs:60-219).
 """
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 
@@ -38,3 +44,54 @@ def renyi_sample(raw: torch.Tensor, uniforms: torch.Tensor, bounds: torch.Tensor
                                        raw.shape[1], guidance, float(alpha), float(cfg), int(offset),
                                        ops._stream(raw)))
     return out[0].view(batch, 1), out[1].view(batch, 1), out[2].view(batch, 1)
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor  # f32 [rows]
+    entropy: torch.Tensor  # f32 [rows], nats
+    rank: torch.Tensor  # int32 [rows], 0 for the best
+    top_ids: torch.Tensor | None  # int32 [rows, top], -1 where there is none
+    top_logprobs: torch.Tensor | None  # f32 [rows, top]
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0, bounds: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None, status: torch.Tensor | None = None) -> TokenLogprobs:
+    """Scores targets (int32 [rows], columns of their rows; -1: none) under
+    logits f32/bf16 [rows, choices] (any row stride): log probability, rank,
+    entropy and the `top` (at most 32) best alternatives.
+
+    bounds, u32 (or i32) [rows, 2] = (start, count) as renyi_sample's, limits
+    each row to a window of legal columns.  A target outside it has log
+    probability -inf and the window's size as its rank.  Alternatives are
+    ordered by (logit descending, column ascending); columns whose logit is
+    -inf are none.  An empty window gives NaN and no alternatives, and so does
+    one outside the choices, which also sets DEV_WINDOW_RANGE in the status
+    word.  NaN or +inf in the window makes log probabilities and entropy NaN.
+    """
+    ops._require_cuda(logits, targets, bounds, workspace, status)
+    if logits.dim() != 2 or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise N.PreconditionError("token logprobs need logits [rows, choices] with contiguous rows and a nonempty head")
+    rows, choices = logits.shape
+    if targets.numel() != rows or targets.dtype != torch.int32 or not targets.is_contiguous():
+        raise N.PreconditionError("token logprobs need one contiguous I32 target a row")
+    if bounds is not None and (bounds.numel() != 2 * rows or bounds.dtype not in (torch.int32, torch.uint32)
+                               or not bounds.is_contiguous()):
+        raise N.PreconditionError("token logprobs bounds must be contiguous U32 [rows, 2]")
+    if not 0 <= top <= 32:
+        raise N.PreconditionError("token logprobs give at most 32 alternatives")
+    code = ops._dtype_code(logits, "logits")
+    stride = logits.stride(0) if rows > 1 else choices
+    dev = logits.device
+    logprob, entropy = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind(0)
+    rank = torch.empty(rows, dtype=torch.int32, device=dev)
+    ids = torch.empty((rows, top), dtype=torch.int32, device=dev) if top else None
+    best = torch.empty((rows, top), dtype=torch.float32, device=dev) if top else None
+    with torch.cuda.device(dev):
+        if workspace is None:
+            need = N.lib.pp_b200_token_logprobs_workspace_size(rows, choices, top)
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        N.check(N.lib.pp_b200_token_logprobs(
+            logits.data_ptr(), code, rows, choices, stride, targets.data_ptr(), ops._ptr(bounds), top,
+            logprob.data_ptr(), entropy.data_ptr(), rank.data_ptr(), ops._ptr(ids), ops._ptr(best), ops._ptr(workspace),
+            workspace.numel() if workspace is not None else 0, ops._ptr(status), ops._stream(logits)))
+    return TokenLogprobs(logprob, entropy, rank, ids, best)
