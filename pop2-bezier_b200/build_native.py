@@ -32,6 +32,7 @@ SOURCES = [
     ("csrc/kernels/sampling.cu", ["-fmad=false", "-prec-div=true", "-prec-sqrt=true"]),
     ("csrc/kernels/lanes.cu", []),
     ("csrc/kernels/prompt.cu", []),
+    ("csrc/kernels/prompt_tc.cu", []),
     ("csrc/kernels/prompt_append.cu", ["-fmad=false", "-prec-div=true", "-prec-sqrt=true"]),
     ("csrc/kernels/logprobs.cu", []),
     ("csrc/host/abi.cpp", []),
@@ -39,7 +40,7 @@ SOURCES = [
     ("csrc/host/sched.cpp", []),
     ("csrc/host/selfcheck.cpp", []),
 ]
-HEADERS = ["csrc/kernels/common.cuh", "csrc/kernels/quant_row.cuh", "csrc/kernels/lanes.cuh", "csrc/kernels/prompt.cuh",
+HEADERS = ["csrc/kernels/common.cuh", "csrc/kernels/quant_row.cuh", "csrc/kernels/lanes.cuh", "csrc/kernels/prompt.cuh", "csrc/kernels/tcgen05.cuh",
            "csrc/host/internal.h"]
 
 

@@ -202,6 +202,9 @@ cudaError_t configure_prompt_kernels();
 int32_t check_arena(const PpKvArena* a, const char* what);
 cudaError_t launch_prompt_plan(const PromptLaunch& L, cudaStream_t stream);
 cudaError_t launch_prompt_rows(const PromptLaunch& L, cudaStream_t stream);
+cudaError_t configure_prompt_tc_kernels();
+cudaError_t launch_prompt_tc(const PromptLaunch& L, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+                             cudaStream_t stream);
 
 // Append of packed prompts: see prompt_append.cu.
 struct PromptAppendLaunch {

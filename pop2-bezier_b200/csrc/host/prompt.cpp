@@ -117,9 +117,29 @@ int32_t pp_b200_prompt_attention(const PpPrompt* prompt, const uint32_t* q_start
             (L.g.k_token_stride * elem) % 16 == 0 && (L.g.k_head_stride * elem) % 16 == 0 &&
             (L.g.v_token_stride * elem) % 16 == 0 && (L.g.v_head_stride * elem) % 16 == 0;
     cudaStream_t st = (cudaStream_t)stream;
+    // The tensor cores take bf16 rows on 16-byte boundaries (what the tensor
+    // copies need; a stride of 0, as `expand` makes, is none they take).
+    const bool tc = L.g.dtype == PP_DTYPE_BF16 && L.vec && L.g.kv_tokens && L.g.q_token_stride && L.g.q_head_stride &&
+                    L.g.k_token_stride && L.g.k_head_stride && L.g.v_token_stride && L.g.v_head_stride;
+    CUtensorMap map_q{}, map_k{}, map_v{};
+    if (tc) {
+        const uint32_t d = L.g.head_dim, group = L.g.heads / L.g.kv_heads;
+        const uint64_t q_dims[4] = {d, group, L.g.q_tokens, L.g.kv_heads};
+        const uint64_t q_st[3] = {L.g.q_head_stride * 2, L.g.q_token_stride * 2, L.g.q_head_stride * 2 * group};
+        const uint32_t q_box[4] = {64, group, 128 / group, 1}, kv_box[3] = {64, 128, 1};
+        const uint64_t kv_dims[3] = {d, L.g.kv_tokens, L.g.kv_heads};
+        const uint64_t k_st[2] = {L.g.k_token_stride * 2, L.g.k_head_stride * 2};
+        const uint64_t v_st[2] = {L.g.v_token_stride * 2, L.g.v_head_stride * 2};
+        const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        if ((s = pp::encode_tiled(&map_q, bf, 4, L.g.q, q_dims, q_st, q_box, "prompt q")) ||
+            (s = pp::encode_tiled(&map_k, bf, 3, L.g.k, kv_dims, k_st, kv_box, "prompt k")) ||
+            (s = pp::encode_tiled(&map_v, bf, 3, L.g.v, kv_dims, v_st, kv_box, "prompt v")))
+            return s;
+    }
     if (!(L.g.flags & PP_ATTN_PLAN_READY) && (s = pp::cuda_status(pp::launch_prompt_plan(L, st), "prompt plan launch")))
         return s;
-    return pp::cuda_status(pp::launch_prompt_rows(L, st), "prompt attention launch");
+    if (!tc) return pp::cuda_status(pp::launch_prompt_rows(L, st), "prompt attention launch");
+    return pp::cuda_status(pp::launch_prompt_tc(L, map_q, map_k, map_v, st), "prompt attention launch");
 }
 
 int32_t pp_b200_prompt_append(const PpKvArena* arena, const void* k, const void* v, int32_t dtype, uint32_t tokens,

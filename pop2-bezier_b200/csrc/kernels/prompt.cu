@@ -523,6 +523,7 @@ PromptArgs prompt_args(const PromptLaunch& L) {
 
 cudaError_t configure_prompt_kernels() {
     cudaError_t e;
+    if ((e = configure_prompt_tc_kernels()) != cudaSuccess) return e;
     if ((e = configure_rows<64, false>()) != cudaSuccess || (e = configure_rows<64, true>()) != cudaSuccess ||
         (e = configure_rows<128, false>()) != cudaSuccess)
         return e;

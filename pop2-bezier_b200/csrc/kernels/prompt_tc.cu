@@ -1,0 +1,647 @@
+// Attention of whole prompts on the tensor cores (bf16, rows on the 16-byte
+// grid): softmax(q k') v of packed sequences, causal or not, grouped heads.
+//
+// One CTA per SM takes work items (prompt.cuh) as it becomes free.  An item is
+// two tiles of 128 query rows against a range of keys in tiles of 128; each
+// tile has a warpgroup of its own for the softmax, so that while one
+// exponentiates, the tensor cores multiply for the other:
+//   warps 0-3, 4-7  softmax of tile 0, 1: a thread owns a row
+//   warp 8          issues the matrix products (tcgen05.mma, one thread)
+//   warp 9          hands out items and loads tiles (TMA, one thread)
+// Tensor memory, 512 columns: the scores S of both tiles (128 each, f32) and
+// their outputs O (head_dim each).  S = Q K' from shared memory; the softmax
+// writes P in bf16 over S, and O += P V reads P from tensor memory.  P in bf16
+// is the tensor cores' operand type; its row sum is taken before the rounding,
+// in f32, as are the maximum and O.
+//
+// The running maximum is a reference point that moves only when a score passes
+// it by 2^8: O is then rescaled in tensor memory, in most key tiles nothing is.
+// A thread may touch O whenever its scores are ready, because S of tile j was
+// issued after P V of tile j - 1 and the tensor cores work in order.
+//
+// Keys that a row does not see get score -inf, hence P = 0, but 0 * v is not 0
+// where v is NaN or infinite (padding, later tokens of the same tile).  Such a
+// row ends up not finite, and its warp computes it again from the keys that it
+// does see.
+#include <math_constants.h>
+
+#include "prompt.cuh"
+#include "tcgen05.cuh"
+
+namespace pp {
+
+PromptArgs prompt_args(const PromptLaunch& L);
+
+namespace {
+
+constexpr int kThreads = 384;
+constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s: generous, never hit in normal runs
+
+template <int D>
+struct TcCfg {
+    static constexpr uint32_t PANEL = 128 * 128;          // 128 rows of 64 bf16
+    static constexpr uint32_t TILE = PANEL * (D / 64);    // a Q, K or V tile
+    static constexpr uint32_t STAGES = D == 128 ? 5 : 8;  // K and V tiles in flight
+    static constexpr uint32_t SMEM = 1024 + 2 * TILE + STAGES * TILE;
+    static constexpr uint32_t S_COL = 0, O_COL = 256;     // tile t: + 128 t, + D t
+};
+
+struct Item {
+    PromptEntry e;
+    uint32_t head, valid;
+};
+
+struct Shared {
+    uint64_t kv_full[8], kv_empty[8];
+    uint64_t q_full[2], q_empty[2];
+    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t item_full[2], item_empty[2];
+    uint64_t group[2];  // a tile's four softmax warps meet
+    uint64_t drain;
+    Item item[2];
+    uint32_t tmem;
+    int abort;
+    int redoing;       // warps that compute rows again: the others wait for them without a limit of their own
+    uint32_t last[2];  // of a tile: this CTA brought the last piece
+    uint32_t spoiled[2];
+};
+
+struct TcMaps {
+    CUtensorMap q, k, v;
+};
+
+// What the roles derive from an item.
+struct Geo {
+    uint32_t tok[2];   // first token of each tile
+    uint32_t live[2];  // rows of each tile that exist
+    uint32_t n[2];     // key tiles each sees
+    uint32_t n_max;
+};
+
+__device__ __forceinline__ Geo geometry_of(const PromptArgs& a, const PromptEntry& e) {
+    Geo g;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        g.tok[t] = e.tok0 + t * a.tpt;
+        const uint32_t tokens = g.tok[t] < e.nq ? min(a.tpt, e.nq - g.tok[t]) : 0u;
+        g.live[t] = tokens * a.group;
+        g.n[t] = 0;
+        if (tokens) {
+            const uint32_t lim = min(e.kv_end, prompt_visible(e, g.tok[t] + tokens - 1, a.causal));
+            if (lim > e.kv_begin) g.n[t] = (lim - e.kv_begin + kPromptKeyTile - 1) / kPromptKeyTile;
+        }
+    }
+    g.n_max = max(g.n[0], g.n[1]);
+    return g;
+}
+
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// A row again, by one warp, from the keys it sees and nothing else (see the top).
+template <int D>
+__device__ __noinline__ void redo_row(const PromptArgs& a, const PromptEntry& e, uint32_t head, uint32_t token,
+                                      uint32_t g) {
+    constexpr int E = D / 32;
+    const int lane = threadIdx.x & 31;
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (uint64_t)(e.q0 + token) * a.q_ts +
+                        (uint64_t)(head * a.group + g) * a.q_hs;
+    const uint32_t end = prompt_visible(e, token, a.causal);
+    float m = -CUDART_INF_F, z = 0.f, acc[E];
+#pragma unroll
+    for (int c = 0; c < E; ++c) acc[c] = 0.f;
+    for (uint32_t n0 = 0; n0 < end; n0 += 32) {
+        float s = -CUDART_INF_F;
+        if (n0 + lane < end) {
+            const uint16_t* k = reinterpret_cast<const uint16_t*>(a.k) + ((uint64_t)e.k0 + n0 + lane) * a.k_ts +
+                                (uint64_t)head * a.k_hs;
+            float dot = 0.f;
+            for (int c = 0; c < D; c += 2) {
+                const uint32_t x = *reinterpret_cast<const uint32_t*>(q + c), y = *reinterpret_cast<const uint32_t*>(k + c);
+                dot = fmaf(bf16_lo_to_f32(x), bf16_lo_to_f32(y), dot);
+                dot = fmaf(bf16_hi_to_f32(x), bf16_hi_to_f32(y), dot);
+            }
+            s = dot * a.scale_log2;
+        }
+        float top = s;
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float mn = fmaxf(m, top), ref = mn == -CUDART_INF_F ? 0.f : mn;
+        const float f = exp2f(m - ref), p = exp2f(s - ref);
+        float sum = p;
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        z = z * f + sum;
+        m = mn;
+#pragma unroll
+        for (int c = 0; c < E; ++c) acc[c] *= f;
+        const uint32_t cnt = min(32u, end - n0);
+        for (uint32_t i = 0; i < cnt; ++i) {
+            const float pi = __shfl_sync(0xffffffffu, p, i);
+            const uint16_t* v = reinterpret_cast<const uint16_t*>(a.v) + ((uint64_t)e.k0 + n0 + i) * a.v_ts +
+                                (uint64_t)head * a.v_hs;
+#pragma unroll
+            for (int c = 0; c < E; ++c) acc[c] = fmaf(pi, bf16_lo_to_f32(v[lane + 32 * c]), acc[c]);
+        }
+    }
+    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) +
+                         ((uint64_t)(e.q0 + token) * a.heads + head * a.group + g) * D;
+#pragma unroll
+    for (int c = 0; c < E; ++c) out[lane + 32 * c] = __float2bfloat16_rn(acc[c] / z);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ TcMaps maps) {
+    using C = TcCfg<D>;
+    extern __shared__ unsigned char raw[];
+    __shared__ Shared sh;
+    unsigned char* smem = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
+    unsigned char* s_q = smem;
+    unsigned char* s_kv = smem + 2 * C::TILE;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int* abort = &sh.abort;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < C::STAGES; ++i) {
+            mbar_init(&sh.kv_full[i], 1);
+            mbar_init(&sh.kv_empty[i], 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&sh.q_full[t], 1);
+            mbar_init(&sh.q_empty[t], 1);
+            mbar_init(&sh.s_full[t], 1);
+            mbar_init(&sh.p_full[t], 4);
+            mbar_init(&sh.o_full[t], 1);
+            mbar_init(&sh.item_full[t], 1);
+            mbar_init(&sh.item_empty[t], 9);
+            mbar_init(&sh.group[t], 4);
+            sh.spoiled[t] = 0;
+        }
+        mbar_init(&sh.drain, 1);
+        fence_mbar_init();
+        sh.abort = 0;
+        sh.redoing = 0;
+        tma_prefetch_desc(&maps.q);
+        tma_prefetch_desc(&maps.k);
+        tma_prefetch_desc(&maps.v);
+    }
+    if (warp == 8) tmem_alloc(&sh.tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    pdl_wait_primary();
+
+    auto give_up = [&] {
+        *abort = 1;
+        if (a.status) atomicOr(a.status, PP_DEV_WAIT_TIMEOUT);
+    };
+    // Whole-warp wait: every lane learns the same answer.
+    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        for (;;) {
+            if (__all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, kWaitLimitNs))) return true;
+            const int busy = *reinterpret_cast<volatile int*>(&sh.redoing);
+            if (__any_sync(0xffffffffu, *abort == 0 && busy > 0)) continue;
+            if (lane == 0) give_up();
+            return false;
+        }
+    };
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 9) {
+            // ------------------------------------------------ items and loads
+            PromptHeader* hdr = reinterpret_cast<PromptHeader*>(a.ws);
+            const PromptEntry* entries = reinterpret_cast<const PromptEntry*>(a.ws + a.l.entries);
+            const uint32_t n_items = hdr->n_items, n_entries = hdr->n_entries;
+            uint32_t it = 0, kv = 0, q_use[2] = {0, 0}, idx = blockIdx.x;
+            const uint32_t q_bytes = a.group * a.tpt * 128 * (D / 64);
+            for (;; ++it) {
+                const uint32_t slot = it & 1;
+                if (!wait(&sh.item_empty[slot], ((it >> 1) & 1) ^ 1)) break;
+                const bool valid = idx < n_items;
+                Item& item = sh.item[slot];
+                uint32_t head = 0;
+                PromptEntry e{};
+                if (valid) {
+                    head = idx / n_entries;
+                    e = entries[idx - head * n_entries];
+                }
+                if (lane == 0) {
+                    item.e = e;
+                    item.head = head;
+                    item.valid = valid;
+                    mbar_arrive(&sh.item_full[slot]);
+                }
+                if (!valid) break;
+                uint32_t next = 0;
+                if (lane == 0) {
+                    next = atomicAdd(&hdr->next, 1u);
+                    if (next == n_items - 1) hdr->next = 0;  // every CTA has taken its last: ready for the next call
+                }
+                const Geo g = geometry_of(a, e);
+                bool ok = true;
+                auto load_q = [&](int t) {
+                    if (!g.n[t] || !ok) return;
+                    if (!(ok = wait(&sh.q_empty[t], (q_use[t] & 1) ^ 1))) return;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&sh.q_full[t], q_bytes);
+                        for (int p = 0; p < D / 64; ++p)
+                            tma_load_4d(s_q + t * C::TILE + p * C::PANEL, &maps.q, &sh.q_full[t], p * 64, 0,
+                                        (int32_t)(e.q0 + g.tok[t]), (int32_t)head);
+                    }
+                    ++q_use[t];
+                };
+                auto load_kv = [&](const CUtensorMap* map, uint32_t j) {
+                    if (!ok) return;
+                    const uint32_t stage = kv % C::STAGES;
+                    if (!(ok = wait(&sh.kv_empty[stage], ((kv / C::STAGES) & 1) ^ 1))) return;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&sh.kv_full[stage], C::TILE);
+                        for (int p = 0; p < D / 64; ++p)
+                            tma_load_3d(s_kv + stage * C::TILE + p * C::PANEL, map, &sh.kv_full[stage], p * 64,
+                                        (int32_t)(e.k0 + e.kv_begin + j * kPromptKeyTile), (int32_t)head);
+                    }
+                    ++kv;
+                };
+                for (uint32_t j = 0; j < g.n_max; ++j) {
+                    if (j == 0) load_q(0);
+                    load_kv(&maps.k, j);
+                    if (j == 0) load_q(1);
+                    load_kv(&maps.v, j);
+                }
+                if (!ok) break;
+                idx = __shfl_sync(0xffffffffu, next, 0) + gridDim.x;
+            }
+            // the loads in flight land before the CTA leaves (a bounded wait each, whatever went wrong)
+            __syncwarp();
+            if (*abort) {
+                int never = 0;
+                for (uint32_t i = kv > C::STAGES ? kv - C::STAGES : 0; i < kv; ++i)
+                    mbar_wait_bounded(&sh.kv_full[i % C::STAGES], (i / C::STAGES) & 1, &never, kWaitLimitNs);
+                for (int t = 0; t < 2; ++t)
+                    if (q_use[t]) mbar_wait_bounded(&sh.q_full[t], (q_use[t] - 1) & 1, &never, kWaitLimitNs);
+            } else {
+                // and so have the tensor cores' arrivals on the ring
+                for (uint32_t i = kv > C::STAGES ? kv - C::STAGES : 0; i < kv; ++i)
+                    if (!wait(&sh.kv_empty[i % C::STAGES], (i / C::STAGES) & 1)) break;
+                for (int t = 0; t < 2; ++t)
+                    if (q_use[t]) wait(&sh.q_empty[t], (q_use[t] - 1) & 1);
+            }
+        } else if (warp == 8) {
+            // --------------------------------------------- the matrix products
+            constexpr uint32_t QK = tc_bf16_desc(128, 128, false), PV = tc_bf16_desc(128, D, true);
+            const uint64_t dq = tc_desc_sw128(smem_addr(s_q), 16, 1024);
+            const uint64_t dk = tc_desc_sw128(smem_addr(s_kv), 16, 1024);
+            const uint64_t dv = tc_desc_sw128(smem_addr(s_kv), C::PANEL, 1024);
+            uint32_t kv = 0, q_use[2] = {0, 0}, p_use[2] = {0, 0};
+            bool ok = true;
+            for (uint32_t it = 0; ok; ++it) {
+                const uint32_t slot = it & 1;
+                if (!wait(&sh.item_full[slot], (it >> 1) & 1)) break;
+                const bool valid = sh.item[slot].valid != 0;
+                const Geo g = geometry_of(a, sh.item[slot].e);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.item_empty[slot]);
+                if (!valid) break;
+                auto full = [&](uint32_t i) { return wait(&sh.kv_full[i % C::STAGES], (i / C::STAGES) & 1); };
+                auto qk = [&](int t, uint32_t i) {  // S_t = Q_t K'
+                    if (lane == 0) {
+                        const uint32_t stage = i % C::STAGES;
+#pragma unroll
+                        for (int c = 0; c < D / 16; ++c) {
+                            const uint32_t off = (c / 4) * C::PANEL + (c % 4) * 32;
+                            tc_mma_ss(tmem + C::S_COL + 128 * t, dq + ((t * C::TILE + off) >> 4),
+                                      dk + ((stage * C::TILE + off) >> 4), QK, c > 0);
+                        }
+                        tc_commit(&sh.s_full[t]);
+                    }
+                };
+                auto pv = [&](int t, uint32_t i, bool first) {  // O_t += P_t V
+                    if (lane == 0) {
+                        const uint32_t stage = i % C::STAGES;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            tc_mma_ts(tmem + C::O_COL + D * t, tmem + C::S_COL + 128 * t + 8 * c,
+                                      dv + ((stage * C::TILE + c * 2048) >> 4), PV, !first || c > 0);
+                    }
+                };
+                // after a tile's last S of the item its Q is free
+                auto q_done = [&](int t) {
+                    if (lane == 0) tc_commit(&sh.q_empty[t]);
+                };
+                if (!g.n_max) continue;
+                ok = full(kv);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (!g.n[t] || !ok) continue;
+                    if (!(ok = wait(&sh.q_full[t], q_use[t]++ & 1))) break;
+                    tc_fence_after();
+                    qk(t, kv);
+                    if (g.n[t] == 1) q_done(t);
+                }
+                if (ok && lane == 0) tc_commit(&sh.kv_empty[kv % C::STAGES]);
+                for (uint32_t j = 0; ok && j < g.n_max; ++j) {
+                    const uint32_t iv = kv + 2 * j + 1, ik = iv + 1;
+                    if (!(ok = full(iv))) break;
+                    bool have_k = false;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (j >= g.n[t] || !ok) continue;
+                        if (!(ok = wait(&sh.p_full[t], p_use[t]++ & 1))) break;
+                        tc_fence_after();
+                        pv(t, iv, j == 0);
+                        if (j + 1 < g.n[t]) {
+                            if (!have_k && !(ok = full(ik))) break;
+                            have_k = true;
+                            tc_fence_after();
+                            qk(t, ik);
+                            if (j + 2 == g.n[t]) q_done(t);
+                        } else if (lane == 0) {
+                            tc_commit(&sh.o_full[t]);
+                        }
+                    }
+                    if (ok && lane == 0) {
+                        tc_commit(&sh.kv_empty[iv % C::STAGES]);
+                        if (j + 1 < g.n_max) tc_commit(&sh.kv_empty[ik % C::STAGES]);
+                    }
+                }
+                kv += 2 * g.n_max;
+            }
+            // no product is running when tensor memory is freed
+            __syncwarp();
+            if (lane == 0) tc_commit(&sh.drain);
+            int never = 0;
+            mbar_wait_bounded(&sh.drain, 0, &never, kWaitLimitNs);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        // ------------------------------------------------------- the softmax
+        const uint32_t t = warp >> 2, r = threadIdx.x & 127, wl = (warp & 3) * 32;
+        const uint32_t s_addr = tmem + (wl << 16) + C::S_COL + 128 * t, o_addr = tmem + (wl << 16) + C::O_COL + D * t;
+        const uint64_t scale2 = f2_pack(a.scale_log2, a.scale_log2);
+        float* acc_ws = reinterpret_cast<float*>(a.ws + a.l.acc);
+        float* ml_ws = reinterpret_cast<float*>(a.ws + a.l.ml);
+        uint32_t* counters = reinterpret_cast<uint32_t*>(a.ws + a.l.counters);
+        uint32_t s_use = 0, o_use = 0, group_use = 0;
+        auto meet = [&]() -> bool {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.group[t]);
+            return wait(&sh.group[t], group_use++ & 1);
+        };
+        for (uint32_t it = 0;; ++it) {
+            const uint32_t slot = it & 1;
+            if (!wait(&sh.item_full[slot], (it >> 1) & 1)) break;
+            const PromptEntry e = sh.item[slot].e;
+            const uint32_t head = sh.item[slot].head, valid = sh.item[slot].valid;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.item_empty[slot]);
+            if (!valid) break;
+            const Geo g = geometry_of(a, e);
+            const uint32_t n = t ? g.n[1] : g.n[0], live_rows = t ? g.live[1] : g.live[0];
+            const uint32_t token = (t ? g.tok[1] : g.tok[0]) + r / a.group, hg = r % a.group;
+            const bool live = r < live_rows;
+            const uint32_t lim = live ? min(e.kv_end, prompt_visible(e, token, a.causal)) : 0u;
+            if (!live_rows) continue;
+            float m = -CUDART_INF_F, z = 0.f;
+            bool ok = true;
+            for (uint32_t j = 0; j < n; ++j) {
+                if (!(ok = wait(&sh.s_full[t], s_use++ & 1))) break;
+                tc_fence_after();
+                uint32_t s[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(reinterpret_cast<uint32_t(&)[32]>(s[32 * c]), s_addr + 32 * c);
+                tmem_wait_ld();
+                const uint32_t n0 = e.kv_begin + j * kPromptKeyTile;
+                const uint32_t see = lim > n0 ? lim - n0 : 0u;  // of this tile
+                if (__any_sync(0xffffffffu, see < kPromptKeyTile)) {
+#pragma unroll
+                    for (int c = 0; c < 128; ++c)
+                        if (c >= see) s[c] = 0xff800000u;
+                }
+                float x0 = __uint_as_float(s[0]), x1 = __uint_as_float(s[1]);
+#pragma unroll
+                for (int c = 2; c < 128; c += 2) {
+                    x0 = fmaxf(x0, __uint_as_float(s[c]));
+                    x1 = fmaxf(x1, __uint_as_float(s[c + 1]));
+                }
+                const float top = fmaxf(x0, x1) * a.scale_log2;
+                const bool moves = top > m + 8.f || (m == -CUDART_INF_F && top > m);
+                if (__any_sync(0xffffffffu, moves)) {
+                    const float mn = moves ? top : m;
+                    const float f = moves ? exp2f(m - mn) : 1.f;
+                    z *= f;
+                    m = mn;
+                    if (j) {
+                        const uint64_t f2 = f2_pack(f, f);
+#pragma unroll
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(o, o_addr + c);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                float lo, hi;
+                                f2_unpack(f2_mul(f2_pack(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), f2), lo, hi);
+                                o[i] = __float_as_uint(lo);
+                                o[i + 1] = __float_as_uint(hi);
+                            }
+                            tmem_st32(o_addr + c, o);
+                        }
+                    }
+                }
+                const float ref = m == -CUDART_INF_F ? 0.f : m;  // nothing seen yet: exp2(-inf) = 0
+                const uint64_t neg = f2_pack(-ref, -ref);
+                uint64_t sum0 = 0ull, sum1 = 0ull;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float lo, hi;
+                        f2_unpack(fma2(f2_pack(__uint_as_float(s[32 * c + 2 * i]), __uint_as_float(s[32 * c + 2 * i + 1])),
+                                       scale2, neg), lo, hi);
+                        lo = fast_exp2(lo);
+                        hi = fast_exp2(hi);
+                        if (i & 1) sum1 = f2_add(sum1, f2_pack(lo, hi));
+                        else sum0 = f2_add(sum0, f2_pack(lo, hi));
+                        p[i] = pack_bf16x2(lo, hi);
+                    }
+                    tmem_st16(s_addr + 16 * c, p);
+                }
+                float lo, hi;
+                f2_unpack(f2_add(sum0, sum1), lo, hi);
+                z += lo + hi;
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.p_full[t]);
+            }
+            if (!ok) break;
+            if (n) {
+                if (!wait(&sh.o_full[t], o_use++ & 1)) break;
+                tc_fence_after();
+            }
+            if (e.n_splits == 1) {
+                const float inv = 1.f / z;  // a row that sees no key: 0 * inf = NaN
+                float chk = 0.f;
+                __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) +
+                                     ((uint64_t)(e.q0 + token) * a.heads + head * a.group + hg) * D;
+#pragma unroll
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    if (n) {
+                        tmem_ld32(o, o_addr + c);
+                        tmem_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = 0u;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        uint4 w;
+                        uint32_t* wp = &w.x;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float x = __uint_as_float(o[i + 2 * k]) * inv, y = __uint_as_float(o[i + 2 * k + 1]) * inv;
+                            chk = fmaf(x, 0.f, chk);
+                            chk = fmaf(y, 0.f, chk);
+                            wp[k] = pack_bf16x2(x, y);
+                        }
+                        if (live) *reinterpret_cast<uint4*>(out + c + i) = w;
+                    }
+                }
+                uint32_t again = __ballot_sync(0xffffffffu, live && lim > 0 && !(chk == 0.f));
+                if (again) {
+                    if (lane == 0) atomicAdd(&sh.redoing, 1);
+                    for (; again; again &= again - 1) {
+                        const int l = __ffs(again) - 1;
+                        redo_row<D>(a, e, head, __shfl_sync(0xffffffffu, token, l), __shfl_sync(0xffffffffu, hg, l));
+                    }
+                    __syncwarp();
+                    if (lane == 0) atomicSub(&sh.redoing, 1);
+                }
+            } else {
+                // partial of this piece; the CTA that brings the last one merges them in the order of the pieces
+                auto slot_row = [&](uint32_t s, uint32_t row) {
+                    return (uint64_t)((e.slot0 + s) * a.kv_heads + head) * a.l.slot_rows + t * kPromptTileRows + row;
+                };
+                const uint64_t at = slot_row(e.split, r);
+                if (n) {
+#pragma unroll
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(o, o_addr + c);
+                        tmem_wait_ld();
+                        if (live) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4)
+                                *reinterpret_cast<uint4*>(acc_ws + at * D + c + i) =
+                                    make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        }
+                    }
+                }
+                if (live) *reinterpret_cast<float2*>(ml_ws + 2 * at) = make_float2(m, z);
+                uint32_t* cnt = counters + 4 * (e.counter * a.kv_heads + head) + t;
+                __threadfence();
+                if (!meet()) break;
+                if (r == 0) sh.last[t] = atomicAdd(cnt, 1u) + 1 == e.n_splits;
+                if (!meet()) break;
+                if (sh.last[t]) {
+                    __threadfence();
+                    if (r == 0) *cnt = 0;
+                    const uint32_t tok0 = t ? g.tok[1] : g.tok[0];
+                    auto out_row = [&](uint32_t row) {
+                        return reinterpret_cast<__nv_bfloat16*>(a.out) +
+                               ((uint64_t)(e.q0 + tok0 + row / a.group) * a.heads + head * a.group + row % a.group) * D;
+                    };
+                    for (uint32_t i = r; i < live_rows * (D / 4); i += 128) {
+                        const uint32_t row = i / (D / 4), c = i % (D / 4) * 4;
+                        float top = -CUDART_INF_F, sum = 0.f;
+                        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (uint32_t s = 0; s < e.n_splits; ++s)
+                            top = fmaxf(top, __ldcg(ml_ws + 2 * slot_row(s, row)));
+                        const float ref = top == -CUDART_INF_F ? 0.f : top;
+                        for (uint32_t s = 0; s < e.n_splits; ++s) {
+                            const uint64_t from = slot_row(s, row);
+                            const float2 mz = __ldcg(reinterpret_cast<const float2*>(ml_ws + 2 * from));
+                            if (mz.y == 0.f) continue;  // the row saw nothing of this piece
+                            const float f = exp2f(mz.x - ref);
+                            const float4 x = __ldcg(reinterpret_cast<const float4*>(acc_ws + from * D + c));
+                            sum += mz.y * f;
+                            o.x += x.x * f;
+                            o.y += x.y * f;
+                            o.z += x.z * f;
+                            o.w += x.w * f;
+                        }
+                        const float inv = 1.f / sum;
+                        o.x *= inv;
+                        o.y *= inv;
+                        o.z *= inv;
+                        o.w *= inv;
+                        *reinterpret_cast<uint2*>(out_row(row) + c) = make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
+                        if (!(o.x * 0.f + o.y * 0.f + o.z * 0.f + o.w * 0.f == 0.f)) sh.spoiled[t] = 1;
+                    }
+                    if (!meet()) break;
+                    if (*reinterpret_cast<volatile uint32_t*>(&sh.spoiled[t])) {
+                        if (lane == 0) atomicAdd(&sh.redoing, 1);
+                        for (uint32_t row = warp & 3; row < live_rows; row += 4) {
+                            const uint16_t* o = reinterpret_cast<const uint16_t*>(out_row(row));
+                            bool bad = false;
+                            for (uint32_t c = lane; c < D; c += 32) bad = bad || (o[c] & 0x7f80u) == 0x7f80u;
+                            if (__any_sync(0xffffffffu, bad)) redo_row<D>(a, e, head, tok0 + row / a.group, row % a.group);
+                        }
+                        __syncwarp();
+                        if (lane == 0) atomicSub(&sh.redoing, 1);
+                        if (!meet()) break;
+                        if (r == 0) sh.spoiled[t] = 0;
+                    }
+                }
+                if (!meet()) break;  // sh.last and sh.spoiled have been read before the next item writes them
+            }
+            tc_fence_before();  // O has been read before the next item's first product may start (p_full)
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+template <int D>
+cudaError_t launch_tc(const PromptArgs& a, const TcMaps& maps, uint32_t ctas, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = TcCfg<D>::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, prompt_tc_kernel<D>, a, maps);
+}
+
+}  // namespace
+
+cudaError_t configure_prompt_tc_kernels() {
+    cudaError_t e = cudaFuncSetAttribute(prompt_tc_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<64>::SMEM);
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(prompt_tc_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<128>::SMEM);
+}
+
+cudaError_t launch_prompt_tc(const PromptLaunch& L, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+                             cudaStream_t stream) {
+    const PromptArgs a = prompt_args(L);
+    TcMaps maps;
+    maps.q = q;
+    maps.k = k;
+    maps.v = v;
+    if (L.g.head_dim == 64) return launch_tc<64>(a, maps, L.layout.max_ctas, stream);
+    return launch_tc<128>(a, maps, L.layout.max_ctas, stream);
+}
+
+}  // namespace pp
