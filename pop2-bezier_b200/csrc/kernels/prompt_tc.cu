@@ -35,7 +35,7 @@ PromptArgs prompt_args(const PromptLaunch& L);
 namespace {
 
 constexpr int kThreads = 384;
-constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s: generous, never hit in normal runs
+constexpr long long kWaitCycles = 4000000000ll;  // 2 s at 2 GHz: generous, never hit in normal runs
 
 template <int D>
 struct TcCfg {
@@ -70,28 +70,23 @@ struct TcMaps {
     CUtensorMap q, k, v;
 };
 
-// What the roles derive from an item.
+// What the roles derive from an item's tile (0 or 1).
 struct Geo {
-    uint32_t tok[2];   // first token of each tile
-    uint32_t live[2];  // rows of each tile that exist
-    uint32_t n[2];     // key tiles each sees
-    uint32_t n_max;
+    uint32_t tok;   // its first token
+    uint32_t live;  // rows of it that exist
+    uint32_t n;     // key tiles it sees
 };
 
-__device__ __forceinline__ Geo geometry_of(const PromptArgs& a, const PromptEntry& e) {
+__device__ __forceinline__ Geo geometry_of(const PromptArgs& a, const PromptEntry& e, uint32_t t) {
     Geo g;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        g.tok[t] = e.tok0 + t * a.tpt;
-        const uint32_t tokens = g.tok[t] < e.nq ? min(a.tpt, e.nq - g.tok[t]) : 0u;
-        g.live[t] = tokens * a.group;
-        g.n[t] = 0;
-        if (tokens) {
-            const uint32_t lim = min(e.kv_end, prompt_visible(e, g.tok[t] + tokens - 1, a.causal));
-            if (lim > e.kv_begin) g.n[t] = (lim - e.kv_begin + kPromptKeyTile - 1) / kPromptKeyTile;
-        }
+    g.tok = e.tok0 + t * a.tpt;
+    const uint32_t tokens = g.tok < e.nq ? min(a.tpt, e.nq - g.tok) : 0u;
+    g.live = tokens * a.group;
+    g.n = 0;
+    if (tokens) {
+        const uint32_t lim = min(e.kv_end, prompt_visible(e, g.tok + tokens - 1, a.causal));
+        if (lim > e.kv_begin) g.n = (lim - e.kv_begin + kPromptKeyTile - 1) / kPromptKeyTile;
     }
-    g.n_max = max(g.n[0], g.n[1]);
     return g;
 }
 
@@ -198,10 +193,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         *abort = 1;
         if (a.status) atomicOr(a.status, PP_DEV_WAIT_TIMEOUT);
     };
-    // Whole-warp wait: every lane learns the same answer.
+    // One thread's wait.
+    auto wait1 = [&](uint64_t* bar, uint32_t parity) -> bool {
+        for (;;) {
+            if (mbar_wait_cycles(bar, parity, abort, kWaitCycles)) return true;
+            if (*abort == 0 && *reinterpret_cast<volatile int*>(&sh.redoing) > 0) continue;
+            give_up();
+            return false;
+        }
+    };
+    // A whole warp's: every lane learns the same answer.
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
         for (;;) {
-            if (__all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, kWaitLimitNs))) return true;
+            if (__all_sync(0xffffffffu, mbar_wait_cycles(bar, parity, abort, kWaitCycles))) return true;
             const int busy = *reinterpret_cast<volatile int*>(&sh.redoing);
             if (__any_sync(0xffffffffu, *abort == 0 && busy > 0)) continue;
             if (lane == 0) give_up();
@@ -211,171 +215,177 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == 9) {
+        if (warp == 9 && lane == 0) {
             // ------------------------------------------------ items and loads
             PromptHeader* hdr = reinterpret_cast<PromptHeader*>(a.ws);
             const PromptEntry* entries = reinterpret_cast<const PromptEntry*>(a.ws + a.l.entries);
             const uint32_t n_items = hdr->n_items, n_entries = hdr->n_entries;
-            uint32_t it = 0, kv = 0, q_use[2] = {0, 0}, idx = blockIdx.x;
             const uint32_t q_bytes = a.group * a.tpt * 128 * (D / 64);
-            for (;; ++it) {
+            uint32_t stage = 0, phase = 0, kv = 0, q_use0 = 0, q_use1 = 0, idx = blockIdx.x;
+            bool ok = true;
+            auto load_q = [&](uint32_t t, uint32_t use, const PromptEntry& e, uint32_t tok, uint32_t head) {
+                if (!ok || !(ok = wait1(&sh.q_empty[t], (use & 1) ^ 1))) return;
+                mbar_arrive_expect_tx(&sh.q_full[t], q_bytes);
+#pragma unroll
+                for (int p = 0; p < D / 64; ++p)
+                    tma_load_4d(s_q + t * C::TILE + p * C::PANEL, &maps.q, &sh.q_full[t], p * 64, 0,
+                                (int32_t)(e.q0 + tok), (int32_t)head);
+            };
+            auto load_kv = [&](const CUtensorMap* map, uint32_t row, uint32_t head) {
+                if (!ok || !(ok = wait1(&sh.kv_empty[stage], phase ^ 1))) return;
+                mbar_arrive_expect_tx(&sh.kv_full[stage], C::TILE);
+#pragma unroll
+                for (int p = 0; p < D / 64; ++p)
+                    tma_load_3d(s_kv + stage * C::TILE + p * C::PANEL, map, &sh.kv_full[stage], p * 64, (int32_t)row,
+                                (int32_t)head);
+                ++kv;
+                if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            };
+            for (uint32_t it = 0; ok; ++it) {
                 const uint32_t slot = it & 1;
-                if (!wait(&sh.item_empty[slot], ((it >> 1) & 1) ^ 1)) break;
-                const bool valid = idx < n_items;
+                if (!(ok = wait1(&sh.item_empty[slot], ((it >> 1) & 1) ^ 1))) break;
                 Item& item = sh.item[slot];
-                uint32_t head = 0;
-                PromptEntry e{};
-                if (valid) {
-                    head = idx / n_entries;
-                    e = entries[idx - head * n_entries];
-                }
-                if (lane == 0) {
-                    item.e = e;
-                    item.head = head;
-                    item.valid = valid;
+                const bool valid = idx < n_items;
+                item.valid = valid;
+                if (!valid) {
                     mbar_arrive(&sh.item_full[slot]);
+                    break;
                 }
-                if (!valid) break;
-                uint32_t next = 0;
-                if (lane == 0) {
-                    next = atomicAdd(&hdr->next, 1u);
-                    if (next == n_items - 1) hdr->next = 0;  // every CTA has taken its last: ready for the next call
+                const uint32_t head = idx / n_entries;
+                const PromptEntry e = entries[idx - head * n_entries];
+                item.e = e;
+                item.head = head;
+                mbar_arrive(&sh.item_full[slot]);
+                const uint32_t next = atomicAdd(&hdr->next, 1u);
+                if (next == n_items - 1) hdr->next = 0;  // every CTA has taken its last: ready for the next call
+                const Geo g0 = geometry_of(a, e, 0), g1 = geometry_of(a, e, 1);
+                const uint32_t n_max = max(g0.n, g1.n);
+                uint32_t row = e.k0 + e.kv_begin;
+                if (g0.n) load_q(0, q_use0++, e, g0.tok, head);
+                if (n_max) load_kv(&maps.k, row, head);
+                if (g1.n) load_q(1, q_use1++, e, g1.tok, head);
+                if (n_max) load_kv(&maps.v, row, head);
+                for (uint32_t j = 1; j < n_max; ++j) {
+                    row += kPromptKeyTile;
+                    load_kv(&maps.k, row, head);
+                    load_kv(&maps.v, row, head);
                 }
-                const Geo g = geometry_of(a, e);
-                bool ok = true;
-                auto load_q = [&](int t) {
-                    if (!g.n[t] || !ok) return;
-                    if (!(ok = wait(&sh.q_empty[t], (q_use[t] & 1) ^ 1))) return;
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(&sh.q_full[t], q_bytes);
-                        for (int p = 0; p < D / 64; ++p)
-                            tma_load_4d(s_q + t * C::TILE + p * C::PANEL, &maps.q, &sh.q_full[t], p * 64, 0,
-                                        (int32_t)(e.q0 + g.tok[t]), (int32_t)head);
-                    }
-                    ++q_use[t];
-                };
-                auto load_kv = [&](const CUtensorMap* map, uint32_t j) {
-                    if (!ok) return;
-                    const uint32_t stage = kv % C::STAGES;
-                    if (!(ok = wait(&sh.kv_empty[stage], ((kv / C::STAGES) & 1) ^ 1))) return;
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(&sh.kv_full[stage], C::TILE);
-                        for (int p = 0; p < D / 64; ++p)
-                            tma_load_3d(s_kv + stage * C::TILE + p * C::PANEL, map, &sh.kv_full[stage], p * 64,
-                                        (int32_t)(e.k0 + e.kv_begin + j * kPromptKeyTile), (int32_t)head);
-                    }
-                    ++kv;
-                };
-                for (uint32_t j = 0; j < g.n_max; ++j) {
-                    if (j == 0) load_q(0);
-                    load_kv(&maps.k, j);
-                    if (j == 0) load_q(1);
-                    load_kv(&maps.v, j);
-                }
-                if (!ok) break;
-                idx = __shfl_sync(0xffffffffu, next, 0) + gridDim.x;
+                idx = next + gridDim.x;
             }
-            // the loads in flight land before the CTA leaves (a bounded wait each, whatever went wrong)
-            __syncwarp();
+            // Before the CTA leaves, the loads in flight have landed (a bounded wait each, whatever went
+            // wrong), and so have the tensor cores' arrivals on the ring.
+            int never = 0;
             if (*abort) {
-                int never = 0;
                 for (uint32_t i = kv > C::STAGES ? kv - C::STAGES : 0; i < kv; ++i)
-                    mbar_wait_bounded(&sh.kv_full[i % C::STAGES], (i / C::STAGES) & 1, &never, kWaitLimitNs);
-                for (int t = 0; t < 2; ++t)
-                    if (q_use[t]) mbar_wait_bounded(&sh.q_full[t], (q_use[t] - 1) & 1, &never, kWaitLimitNs);
+                    mbar_wait_cycles(&sh.kv_full[i % C::STAGES], (i / C::STAGES) & 1, &never, kWaitCycles);
+                if (q_use0) mbar_wait_cycles(&sh.q_full[0], (q_use0 - 1) & 1, &never, kWaitCycles);
+                if (q_use1) mbar_wait_cycles(&sh.q_full[1], (q_use1 - 1) & 1, &never, kWaitCycles);
             } else {
-                // and so have the tensor cores' arrivals on the ring
-                for (uint32_t i = kv > C::STAGES ? kv - C::STAGES : 0; i < kv; ++i)
-                    if (!wait(&sh.kv_empty[i % C::STAGES], (i / C::STAGES) & 1)) break;
-                for (int t = 0; t < 2; ++t)
-                    if (q_use[t]) wait(&sh.q_empty[t], (q_use[t] - 1) & 1);
+                for (uint32_t i = kv > C::STAGES ? kv - C::STAGES : 0; ok && i < kv; ++i)
+                    ok = wait1(&sh.kv_empty[i % C::STAGES], (i / C::STAGES) & 1);
+                if (q_use0 && ok) ok = wait1(&sh.q_empty[0], (q_use0 - 1) & 1);
+                if (q_use1 && ok) ok = wait1(&sh.q_empty[1], (q_use1 - 1) & 1);
             }
-        } else if (warp == 8) {
+        } else if (warp == 8 && lane == 0) {
             // --------------------------------------------- the matrix products
             constexpr uint32_t QK = tc_bf16_desc(128, 128, false), PV = tc_bf16_desc(128, D, true);
             const uint64_t dq = tc_desc_sw128(smem_addr(s_q), 16, 1024);
             const uint64_t dk = tc_desc_sw128(smem_addr(s_kv), 16, 1024);
             const uint64_t dv = tc_desc_sw128(smem_addr(s_kv), C::PANEL, 1024);
-            uint32_t kv = 0, q_use[2] = {0, 0}, p_use[2] = {0, 0};
+            uint32_t stage = 0, phase = 0, q_use0 = 0, q_use1 = 0, p_use0 = 0, p_use1 = 0;
             bool ok = true;
+            auto advance = [&] {
+                if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            };
+            auto qk = [&](uint32_t t, uint32_t st) {  // S_t = Q_t K'
+                const uint64_t da = dq + (t * C::TILE >> 4), db = dk + (st * C::TILE >> 4);
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c)
+                    tc_mma_ss(tmem + C::S_COL + 128 * t, da + (((c / 4) * C::PANEL + (c % 4) * 32) >> 4),
+                              db + (((c / 4) * C::PANEL + (c % 4) * 32) >> 4), QK, c > 0);
+                tc_commit(&sh.s_full[t]);
+            };
+            auto pv = [&](uint32_t t, uint32_t st, bool first) {  // O_t += P_t V
+                const uint64_t db = dv + (st * C::TILE >> 4);
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    tc_mma_ts(tmem + C::O_COL + D * t, tmem + C::S_COL + 128 * t + 8 * c, db + (c * 2048 >> 4), PV,
+                              !first || c > 0);
+            };
             for (uint32_t it = 0; ok; ++it) {
                 const uint32_t slot = it & 1;
-                if (!wait(&sh.item_full[slot], (it >> 1) & 1)) break;
+                if (!(ok = wait1(&sh.item_full[slot], (it >> 1) & 1))) break;
                 const bool valid = sh.item[slot].valid != 0;
-                const Geo g = geometry_of(a, sh.item[slot].e);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.item_empty[slot]);
+                const PromptEntry& e = sh.item[slot].e;
+                const uint32_t n0 = valid ? geometry_of(a, e, 0).n : 0u, n1 = valid ? geometry_of(a, e, 1).n : 0u;
+                const uint32_t n_max = max(n0, n1);
+                mbar_arrive(&sh.item_empty[slot]);
                 if (!valid) break;
-                auto full = [&](uint32_t i) { return wait(&sh.kv_full[i % C::STAGES], (i / C::STAGES) & 1); };
-                auto qk = [&](int t, uint32_t i) {  // S_t = Q_t K'
-                    if (lane == 0) {
-                        const uint32_t stage = i % C::STAGES;
-#pragma unroll
-                        for (int c = 0; c < D / 16; ++c) {
-                            const uint32_t off = (c / 4) * C::PANEL + (c % 4) * 32;
-                            tc_mma_ss(tmem + C::S_COL + 128 * t, dq + ((t * C::TILE + off) >> 4),
-                                      dk + ((stage * C::TILE + off) >> 4), QK, c > 0);
-                        }
-                        tc_commit(&sh.s_full[t]);
-                    }
-                };
-                auto pv = [&](int t, uint32_t i, bool first) {  // O_t += P_t V
-                    if (lane == 0) {
-                        const uint32_t stage = i % C::STAGES;
-#pragma unroll
-                        for (int c = 0; c < 8; ++c)
-                            tc_mma_ts(tmem + C::O_COL + D * t, tmem + C::S_COL + 128 * t + 8 * c,
-                                      dv + ((stage * C::TILE + c * 2048) >> 4), PV, !first || c > 0);
-                    }
-                };
-                // after a tile's last S of the item its Q is free
-                auto q_done = [&](int t) {
-                    if (lane == 0) tc_commit(&sh.q_empty[t]);
-                };
-                if (!g.n_max) continue;
-                ok = full(kv);
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (!g.n[t] || !ok) continue;
-                    if (!(ok = wait(&sh.q_full[t], q_use[t]++ & 1))) break;
+                if (!n_max) continue;
+                // S of the first key tile; after a tile's last S of the item its Q is free
+                if (!(ok = wait1(&sh.kv_full[stage], phase))) break;
+                if (n0) {
+                    if (!(ok = wait1(&sh.q_full[0], q_use0++ & 1))) break;
                     tc_fence_after();
-                    qk(t, kv);
-                    if (g.n[t] == 1) q_done(t);
+                    qk(0, stage);
+                    if (n0 == 1) tc_commit(&sh.q_empty[0]);
                 }
-                if (ok && lane == 0) tc_commit(&sh.kv_empty[kv % C::STAGES]);
-                for (uint32_t j = 0; ok && j < g.n_max; ++j) {
-                    const uint32_t iv = kv + 2 * j + 1, ik = iv + 1;
-                    if (!(ok = full(iv))) break;
-                    bool have_k = false;
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        if (j >= g.n[t] || !ok) continue;
-                        if (!(ok = wait(&sh.p_full[t], p_use[t]++ & 1))) break;
+                if (n1) {
+                    if (!(ok = wait1(&sh.q_full[1], q_use1++ & 1))) break;
+                    tc_fence_after();
+                    qk(1, stage);
+                    if (n1 == 1) tc_commit(&sh.q_empty[1]);
+                }
+                tc_commit(&sh.kv_empty[stage]);
+                advance();
+                for (uint32_t j = 0; j < n_max; ++j) {
+                    const uint32_t sv = stage, pv_phase = phase;
+                    advance();
+                    const uint32_t sk = stage, pk_phase = phase;
+                    const bool more = j + 1 < n_max;
+                    if (!(ok = wait1(&sh.kv_full[sv], pv_phase))) break;
+                    if (more && !(ok = wait1(&sh.kv_full[sk], pk_phase))) break;
+                    if (j < n0) {
+                        if (!(ok = wait1(&sh.p_full[0], p_use0++ & 1))) break;
                         tc_fence_after();
-                        pv(t, iv, j == 0);
-                        if (j + 1 < g.n[t]) {
-                            if (!have_k && !(ok = full(ik))) break;
-                            have_k = true;
-                            tc_fence_after();
-                            qk(t, ik);
-                            if (j + 2 == g.n[t]) q_done(t);
-                        } else if (lane == 0) {
-                            tc_commit(&sh.o_full[t]);
+                        pv(0, sv, j == 0);
+                        if (j + 1 < n0) {
+                            qk(0, sk);
+                            if (j + 2 == n0) tc_commit(&sh.q_empty[0]);
+                        } else {
+                            tc_commit(&sh.o_full[0]);
                         }
                     }
-                    if (ok && lane == 0) {
-                        tc_commit(&sh.kv_empty[iv % C::STAGES]);
-                        if (j + 1 < g.n_max) tc_commit(&sh.kv_empty[ik % C::STAGES]);
+                    if (j < n1) {
+                        if (!(ok = wait1(&sh.p_full[1], p_use1++ & 1))) break;
+                        tc_fence_after();
+                        pv(1, sv, j == 0);
+                        if (j + 1 < n1) {
+                            qk(1, sk);
+                            if (j + 2 == n1) tc_commit(&sh.q_empty[1]);
+                        } else {
+                            tc_commit(&sh.o_full[1]);
+                        }
+                    }
+                    tc_commit(&sh.kv_empty[sv]);
+                    if (more) {
+                        tc_commit(&sh.kv_empty[sk]);
+                        advance();
                     }
                 }
-                kv += 2 * g.n_max;
             }
             // no product is running when tensor memory is freed
-            __syncwarp();
-            if (lane == 0) tc_commit(&sh.drain);
+            tc_commit(&sh.drain);
             int never = 0;
-            mbar_wait_bounded(&sh.drain, 0, &never, kWaitLimitNs);
+            mbar_wait_cycles(&sh.drain, 0, &never, kWaitCycles);
         }
+        __syncwarp();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ------------------------------------------------------- the softmax
@@ -399,9 +409,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.item_empty[slot]);
             if (!valid) break;
-            const Geo g = geometry_of(a, e);
-            const uint32_t n = t ? g.n[1] : g.n[0], live_rows = t ? g.live[1] : g.live[0];
-            const uint32_t token = (t ? g.tok[1] : g.tok[0]) + r / a.group, hg = r % a.group;
+            const Geo g = geometry_of(a, e, t);
+            const uint32_t n = g.n, live_rows = g.live;
+            const uint32_t token = g.tok + r / a.group, hg = r % a.group;
             const bool live = r < live_rows;
             const uint32_t lim = live ? min(e.kv_end, prompt_visible(e, token, a.causal)) : 0u;
             if (!live_rows) continue;
@@ -552,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (sh.last[t]) {
                     __threadfence();
                     if (r == 0) *cnt = 0;
-                    const uint32_t tok0 = t ? g.tok[1] : g.tok[0];
+                    const uint32_t tok0 = g.tok;
                     auto out_row = [&](uint32_t row) {
                         return reinterpret_cast<__nv_bfloat16*>(a.out) +
                                ((uint64_t)(e.q0 + tok0 + row / a.group) * a.heads + head * a.group + row % a.group) * D;

@@ -30,6 +30,18 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
                  : "memory");
 }
 
+// mbar_wait_bounded with the limit in SM clock cycles: %globaltimer takes about
+// a microsecond to read, which a wait that is over after a few hundred cycles
+// would feel at every key tile.
+__device__ __forceinline__ bool mbar_wait_cycles(uint64_t* bar, uint32_t parity, volatile int* abort, long long limit) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long start = clock64();
+    for (uint32_t n = 1;; ++n) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((n & 63u) == 0 && (*abort || clock64() - start > limit)) return false;
+    }
+}
+
 // bf16 operands, f32 accumulator: A [M, K] K-major, B [N, K] K-major or (mn) [K, N].
 __host__ __device__ constexpr uint32_t tc_bf16_desc(uint32_t m, uint32_t n, bool b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
