@@ -10,13 +10,17 @@ namespace {
 // ----------------------------------------------------------------- the plan
 //
 // One CTA.  Cuts every sequence into entries of 2 * tpt query tokens, counts
-// the key tiles each sees, and writes them longest first (64 classes of
-// length), because the attention CTAs take items in this order as they become
-// free: the last ones taken are the shortest.  Where the whole batch has fewer
-// key tiles than it takes to keep every CTA busy with whole entries, an entry
-// longer than its share is cut into equal pieces along the keys.
+// the steps each takes (a step is a key tile of both its query tiles, or two
+// key tiles where only one has rows), and writes them longest first (64 classes
+// of length), because the attention CTAs take items in this order as they
+// become free: the last ones taken are the shortest.  Where the whole batch has
+// fewer steps than it takes to keep every CTA busy with whole entries, an entry
+// of more than one and a half times its share is cut into equal pieces along
+// the keys; below that, the merge and the uneven last round cost what the cut
+// gains.
 constexpr int kPlanThreads = 1024;
 constexpr uint32_t kClasses = 64;
+constexpr uint32_t kBaseMax = 2048;  // sequences whose first entries are kept in shared memory
 #ifndef PP_PROMPT_MIN_SHARE
 #define PP_PROMPT_MIN_SHARE 2
 #endif
@@ -56,14 +60,20 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* warp_tot, u
     return inc - x + (w ? warp_tot[w - 1] : 0u);
 }
 
-// Entry `e` before cutting: its sequence and the number of key tiles it sees.
-__device__ __forceinline__ uint32_t entry_of(const PlanArgs& a, const uint32_t* seq_base, uint32_t e, PromptEntry& p) {
+struct Whole {  // an entry before cutting
+    PromptEntry p;
+    uint32_t tiles, steps;
+};
+
+__device__ __forceinline__ Whole entry_of(const PlanArgs& a, const uint32_t* seq_base, uint32_t e) {
+    Whole w;
     uint32_t lo = 0, hi = a.sequences;  // seq_base[lo] <= e < seq_base[hi]
     while (hi - lo > 1) {
         const uint32_t mid = lo + (hi - lo) / 2;
         if (seq_base[mid] <= e) lo = mid;
         else hi = mid;
     }
+    PromptEntry& p = w.p;
     p.q0 = a.q_starts[lo];
     p.nq = a.q_starts[lo + 1] - p.q0;
     p.k0 = a.kv_starts[lo];
@@ -71,74 +81,87 @@ __device__ __forceinline__ uint32_t entry_of(const PlanArgs& a, const uint32_t* 
     p.tok0 = (e - seq_base[lo]) * 2 * a.tpt;
     p.kv_begin = 0;
     p.kv_end = prompt_visible(p, min(p.nq, p.tok0 + 2 * a.tpt) - 1, a.causal);
-    return max(1u, (uint32_t)(((uint64_t)p.kv_end + kPromptKeyTile - 1) / kPromptKeyTile));
+    w.tiles = max(1u, p.kv_end / kPromptKeyTile + (p.kv_end % kPromptKeyTile != 0));
+    w.steps = p.tok0 + a.tpt >= p.nq ? (w.tiles + 1) / 2 : w.tiles;
+    return w;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArgs a) {
-    __shared__ uint32_t warp_tot[32], hist[kClasses], cursor[kClasses];
-    __shared__ uint32_t bad, longest, slots, cuts;
-    __shared__ unsigned long long work;
-    const uint32_t t = threadIdx.x;
+    __shared__ uint32_t warp_tot[32], hist[kClasses], cursor[kClasses], base_s[kBaseMax + 1];
+    __shared__ unsigned long long warp_work[32];
+    __shared__ uint32_t longest, slots, cuts;
+    const uint32_t t = threadIdx.x, lane = t & 31;
     PromptHeader* hdr = reinterpret_cast<PromptHeader*>(a.ws);
-    uint32_t* seq_base = reinterpret_cast<uint32_t*>(a.ws + a.l.seq_base);
+    uint32_t* seq_base = a.sequences <= kBaseMax ? base_s : reinterpret_cast<uint32_t*>(a.ws + a.l.seq_base);
     PromptEntry* entries = reinterpret_cast<PromptEntry*>(a.ws + a.l.entries);
     uint32_t* counters = reinterpret_cast<uint32_t*>(a.ws + a.l.counters);
-    if (t == 0) {
-        bad = longest = slots = cuts = 0;
-        work = 0;
-    }
+    if (t == 0) longest = slots = cuts = 0;
     if (t < kClasses) hist[t] = 0;
     // launched as a programmatic dependent: the kernels before may still read
     // the workspace or write the starts.  A dependent attention launch may
     // start now; it waits for this kernel before it reads the plan.
     pdl_wait_primary();
     pdl_launch_dependents();
-    __syncthreads();
     for (uint32_t i = t; i < 4 * a.l.max_ctas; i += kPlanThreads) counters[i] = 0;
-    for (uint32_t b = t; b < a.sequences; b += kPlanThreads) {
-        const uint32_t q0 = a.q_starts[b], q1 = a.q_starts[b + 1], k0 = a.kv_starts[b], k1 = a.kv_starts[b + 1];
-        if (q1 < q0 || q1 > a.q_tokens || k1 < k0 || k1 > a.kv_tokens) bad = 1;
-    }
-    __syncthreads();
+    int bad = 0;
     uint32_t n = 0;
-    if (!bad) {
-        for (uint32_t b0 = 0; b0 < a.sequences; b0 += kPlanThreads) {
-            const uint32_t b = b0 + t;
-            const uint32_t nq = b < a.sequences ? a.q_starts[b + 1] - a.q_starts[b] : 0u;
-            uint32_t tot;
-            const uint32_t at = block_scan(nq / (2 * a.tpt) + (nq % (2 * a.tpt) != 0), warp_tot, tot);
-            if (b < a.sequences) seq_base[b] = n + at;
-            n += tot;
+    for (uint32_t b0 = 0; b0 < a.sequences; b0 += kPlanThreads) {
+        const uint32_t b = b0 + t;
+        uint32_t nq = 0;
+        if (b < a.sequences) {
+            const uint32_t q0 = a.q_starts[b], q1 = a.q_starts[b + 1], k0 = a.kv_starts[b], k1 = a.kv_starts[b + 1];
+            if (q1 < q0 || q1 > a.q_tokens || k1 < k0 || k1 > a.kv_tokens) bad = 1;
+            else nq = q1 - q0;
         }
+        uint32_t tot;
+        const uint32_t at = block_scan(nq / (2 * a.tpt) + (nq % (2 * a.tpt) != 0), warp_tot, tot);
+        if (b < a.sequences) seq_base[b] = n + at;
+        n += tot;
     }
-    if (t == 0) {
-        seq_base[a.sequences] = n;
-        if (bad && a.status) atomicOr(a.status, PP_DEV_LENGTH_RANGE);
+    if (__syncthreads_or(bad)) {
+        n = 0;
+        if (t == 0 && a.status) atomicOr(a.status, PP_DEV_LENGTH_RANGE);
     }
+    if (t == 0) seq_base[a.sequences] = n;
     __syncthreads();
+    Whole first;  // the thread's first entry, often its only one
+    if (t < n) first = entry_of(a, seq_base, t);
     {
         unsigned long long mine = 0;
         uint32_t far = 0;
         for (uint32_t e = t; e < n; e += kPlanThreads) {
-            PromptEntry p;
-            const uint32_t tiles = entry_of(a, seq_base, e, p);
-            mine += tiles;
-            far = max(far, tiles);
+            const uint32_t steps = e == t ? first.steps : entry_of(a, seq_base, e).steps;
+            mine += steps;
+            far = max(far, steps);
         }
-        if (far) {
-            atomicAdd(&work, mine);
-            atomicMax(&longest, far);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            mine += __shfl_xor_sync(0xffffffffu, mine, o);
+            far = max(far, __shfl_xor_sync(0xffffffffu, far, o));
+        }
+        if (lane == 0) {
+            warp_work[t >> 5] = mine;
+            if (far) atomicMax(&longest, far);
         }
     }
     __syncthreads();
-    const unsigned long long all = work * a.kv_heads;
-    const uint32_t share = (uint32_t)max((unsigned long long)PP_PROMPT_MIN_SHARE, (all + a.l.max_ctas - 1) / a.l.max_ctas);
-    const uint32_t most = min(longest, share);  // key tiles of the longest piece
+    unsigned long long all = warp_work[lane];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    all *= a.kv_heads;
+    const unsigned long long share = (all + a.l.max_ctas - 1) / a.l.max_ctas;
+    const uint32_t limit = (uint32_t)max((unsigned long long)PP_PROMPT_MIN_SHARE, min(share + share / 2, 0x7fffffffull));
+    const uint32_t most = min(longest, limit);  // steps of the longest piece
+    // pieces of an entry and the class of their length (steps < 2^25, so the product fits)
+    auto cut = [&](const Whole& w, uint32_t& pieces) {
+        pieces = (w.steps + limit - 1) / limit;
+        const uint32_t len = (w.steps + pieces - 1) / pieces;
+        return kClasses - 1 - (len - 1) * kClasses / most;
+    };
     for (uint32_t e = t; e < n; e += kPlanThreads) {
-        PromptEntry p;
-        const uint32_t tiles = entry_of(a, seq_base, e, p);
-        const uint32_t pieces = (tiles + share - 1) / share, len = (tiles + pieces - 1) / pieces;
-        atomicAdd(&hist[kClasses - 1 - (uint32_t)((uint64_t)(len - 1) * kClasses / most)], pieces);
+        uint32_t pieces;
+        const uint32_t c = e == t ? cut(first, pieces) : cut(entry_of(a, seq_base, e), pieces);
+        atomicAdd(&hist[c], pieces);
     }
     __syncthreads();
     if (t < 32) {
@@ -158,10 +181,10 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
     }
     __syncthreads();
     for (uint32_t e = t; e < n; e += kPlanThreads) {
-        PromptEntry p;
-        const uint32_t tiles = entry_of(a, seq_base, e, p);
-        const uint32_t pieces = (tiles + share - 1) / share, len = (tiles + pieces - 1) / pieces;
-        uint32_t at = atomicAdd(&cursor[kClasses - 1 - (uint32_t)((uint64_t)(len - 1) * kClasses / most)], pieces);
+        Whole w = e == t ? first : entry_of(a, seq_base, e);
+        uint32_t pieces;
+        const uint32_t at = atomicAdd(&cursor[cut(w, pieces)], pieces);
+        PromptEntry p = w.p;
         p.n_splits = pieces;
         p.slot0 = p.counter = p.pad = 0;
         if (pieces > 1) {
@@ -172,8 +195,8 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
         for (uint32_t s = 0; s < pieces; ++s) {
             // equal pieces of whole tiles: none is empty, as s * tiles / pieces is strictly increasing
             p.split = s;
-            p.kv_begin = (uint32_t)((uint64_t)tiles * s / pieces) * kPromptKeyTile;
-            p.kv_end = s + 1 == pieces ? end : (uint32_t)((uint64_t)tiles * (s + 1) / pieces) * kPromptKeyTile;
+            p.kv_begin = (uint32_t)((uint64_t)w.tiles * s / pieces) * kPromptKeyTile;
+            p.kv_end = s + 1 == pieces ? end : (uint32_t)((uint64_t)w.tiles * (s + 1) / pieces) * kPromptKeyTile;
             entries[at + s] = p;
         }
     }

@@ -19,6 +19,12 @@
 // A thread may touch O whenever its scores are ready, because S of tile j was
 // issued after P V of tile j - 1 and the tensor cores work in order.
 //
+// Where only tile 0 has rows (single tokens, short chunks), both warpgroups take
+// them, each half of the key tiles with its own maximum, sum and output; at the
+// end the first merges the two, both being in its tensor memory lanes.  Such an
+// item is bound by the latency of one tile's chain (S, softmax, P V), and two
+// chains side by side halve it.
+//
 // Keys that a row does not see get score -inf, hence P = 0, but 0 * v is not 0
 // where v is NaN or infinite (padding, later tokens of the same tile).  Such a
 // row ends up not finite, and its warp computes it again from the keys that it
@@ -63,7 +69,8 @@ struct Shared {
     int abort;
     int redoing;       // warps that compute rows again: the others wait for them without a limit of their own
     uint32_t last[2];  // of a tile: this CTA brought the last piece
-    uint32_t spoiled[2];
+    uint64_t half_full, half_empty;  // the second half of a shared tile is there, has been merged
+    float2 half[128];                // its maximum and sum
 };
 
 struct TcMaps {
@@ -72,20 +79,32 @@ struct TcMaps {
 
 // What the roles derive from an item's tile (0 or 1).
 struct Geo {
-    uint32_t tok;   // its first token
-    uint32_t live;  // rows of it that exist
-    uint32_t n;     // key tiles it sees
+    uint32_t tok;    // its first token
+    uint32_t live;   // rows of it that exist
+    uint32_t first;  // its first key
+    uint32_t n;      // key tiles it sees from there on
+    bool halves;     // tile 1 stands for tile 0's rows and the second half of their key tiles
 };
 
 __device__ __forceinline__ Geo geometry_of(const PromptArgs& a, const PromptEntry& e, uint32_t t) {
     Geo g;
-    g.tok = e.tok0 + t * a.tpt;
+    const bool single = e.tok0 + a.tpt >= e.nq;
+    g.tok = e.tok0 + (single ? 0u : t * a.tpt);
     const uint32_t tokens = g.tok < e.nq ? min(a.tpt, e.nq - g.tok) : 0u;
     g.live = tokens * a.group;
+    g.first = e.kv_begin;
     g.n = 0;
     if (tokens) {
         const uint32_t lim = min(e.kv_end, prompt_visible(e, g.tok + tokens - 1, a.causal));
         if (lim > e.kv_begin) g.n = (lim - e.kv_begin + kPromptKeyTile - 1) / kPromptKeyTile;
+    }
+    g.halves = single && g.n > 1;
+    if (g.halves) {
+        const uint32_t low = (g.n + 1) / 2;
+        if (t) g.first += low * kPromptKeyTile;
+        g.n = t ? g.n - low : low;
+    } else if (single && t) {
+        g.live = g.n = 0;
     }
     return g;
 }
@@ -94,6 +113,12 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
+}
+
+__device__ __forceinline__ void st_global_v8(float* p, const uint32_t* v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 
 // A row again, by one warp, from the keys it sees and nothing else (see the top).
@@ -172,9 +197,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&sh.item_full[t], 1);
             mbar_init(&sh.item_empty[t], 9);
             mbar_init(&sh.group[t], 4);
-            sh.spoiled[t] = 0;
         }
         mbar_init(&sh.drain, 1);
+        mbar_init(&sh.half_full, 4);
+        mbar_init(&sh.half_empty, 4);
         fence_mbar_init();
         sh.abort = 0;
         sh.redoing = 0;
@@ -263,7 +289,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (next == n_items - 1) hdr->next = 0;  // every CTA has taken its last: ready for the next call
                 const Geo g0 = geometry_of(a, e, 0), g1 = geometry_of(a, e, 1);
                 const uint32_t n_max = max(g0.n, g1.n);
-                uint32_t row = e.k0 + e.kv_begin;
+                uint32_t row = e.k0 + g0.first;
+                if (g0.halves) {  // in the order of the products below
+                    const uint32_t row1 = e.k0 + g1.first;
+                    load_q(0, q_use0++, e, g0.tok, head);
+                    load_kv(&maps.k, row, head);
+                    load_q(1, q_use1++, e, g0.tok, head);
+                    load_kv(&maps.k, row1, head);
+                    for (uint32_t j = 0; j < g0.n; ++j) {
+                        load_kv(&maps.v, row + j * kPromptKeyTile, head);
+                        if (j + 1 < g0.n) load_kv(&maps.k, row + (j + 1) * kPromptKeyTile, head);
+                        if (j < g1.n) load_kv(&maps.v, row1 + j * kPromptKeyTile, head);
+                        if (j + 1 < g1.n) load_kv(&maps.k, row1 + (j + 1) * kPromptKeyTile, head);
+                    }
+                    idx = next + gridDim.x;
+                    continue;
+                }
                 if (g0.n) load_q(0, q_use0++, e, g0.tok, head);
                 if (n_max) load_kv(&maps.k, row, head);
                 if (g1.n) load_q(1, q_use1++, e, g1.tok, head);
@@ -323,11 +364,64 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = wait1(&sh.item_full[slot], (it >> 1) & 1))) break;
                 const bool valid = sh.item[slot].valid != 0;
                 const PromptEntry& e = sh.item[slot].e;
-                const uint32_t n0 = valid ? geometry_of(a, e, 0).n : 0u, n1 = valid ? geometry_of(a, e, 1).n : 0u;
+                uint32_t n0 = 0, n1 = 0;
+                bool halves = false;
+                if (valid) {
+                    const Geo g0 = geometry_of(a, e, 0);
+                    n0 = g0.n;
+                    halves = g0.halves;
+                    n1 = geometry_of(a, e, 1).n;
+                }
                 const uint32_t n_max = max(n0, n1);
                 mbar_arrive(&sh.item_empty[slot]);
                 if (!valid) break;
                 if (!n_max) continue;
+                if (halves) {  // the two chains share nothing but Q's rows; n1 is n0 or n0 - 1
+                    auto next_full = [&] { return wait1(&sh.kv_full[stage], phase); };
+                    auto release = [&] {
+                        tc_commit(&sh.kv_empty[stage]);
+                        advance();
+                    };
+                    if (!(ok = wait1(&sh.q_full[0], q_use0++ & 1) && next_full())) break;
+                    tc_fence_after();
+                    qk(0, stage);
+                    if (n0 == 1) tc_commit(&sh.q_empty[0]);
+                    release();
+                    if (!(ok = wait1(&sh.q_full[1], q_use1++ & 1) && next_full())) break;
+                    tc_fence_after();
+                    qk(1, stage);
+                    if (n1 == 1) tc_commit(&sh.q_empty[1]);
+                    release();
+                    for (uint32_t j = 0; ok && j < n0; ++j) {
+                        if (!(ok = next_full() && wait1(&sh.p_full[0], p_use0++ & 1))) break;
+                        tc_fence_after();
+                        pv(0, stage, j == 0);
+                        release();
+                        if (j + 1 < n0) {
+                            if (!(ok = next_full())) break;
+                            qk(0, stage);
+                            if (j + 2 == n0) tc_commit(&sh.q_empty[0]);
+                            release();
+                        } else {
+                            tc_commit(&sh.o_full[0]);
+                        }
+                        if (j < n1) {
+                            if (!(ok = next_full() && wait1(&sh.p_full[1], p_use1++ & 1))) break;
+                            tc_fence_after();
+                            pv(1, stage, j == 0);
+                            release();
+                            if (j + 1 < n1) {
+                                if (!(ok = next_full())) break;
+                                qk(1, stage);
+                                if (j + 2 == n1) tc_commit(&sh.q_empty[1]);
+                                release();
+                            } else {
+                                tc_commit(&sh.o_full[1]);
+                            }
+                        }
+                    }
+                    continue;
+                }
                 // S of the first key tile; after a tile's last S of the item its Q is free
                 if (!(ok = wait1(&sh.kv_full[stage], phase))) break;
                 if (n0) {
@@ -395,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float* acc_ws = reinterpret_cast<float*>(a.ws + a.l.acc);
         float* ml_ws = reinterpret_cast<float*>(a.ws + a.l.ml);
         uint32_t* counters = reinterpret_cast<uint32_t*>(a.ws + a.l.counters);
-        uint32_t s_use = 0, o_use = 0, group_use = 0;
+        uint32_t s_use = 0, o_use = 0, group_use = 0, half_use = 0;
         auto meet = [&]() -> bool {
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.group[t]);
@@ -411,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!valid) break;
             const Geo g = geometry_of(a, e, t);
             const uint32_t n = g.n, live_rows = g.live;
-            const uint32_t token = g.tok + r / a.group, hg = r % a.group;
+            const uint32_t token = g.tok + r / a.group;
             const bool live = r < live_rows;
             const uint32_t lim = live ? min(e.kv_end, prompt_visible(e, token, a.causal)) : 0u;
             if (!live_rows) continue;
@@ -424,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_ld32(reinterpret_cast<uint32_t(&)[32]>(s[32 * c]), s_addr + 32 * c);
                 tmem_wait_ld();
-                const uint32_t n0 = e.kv_begin + j * kPromptKeyTile;
+                const uint32_t n0 = g.first + j * kPromptKeyTile;
                 const uint32_t see = lim > n0 ? lim - n0 : 0u;  // of this tile
                 if (__any_sync(0xffffffffu, see < kPromptKeyTile)) {
 #pragma unroll
@@ -494,63 +588,86 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!wait(&sh.o_full[t], o_use++ & 1)) break;
                 tc_fence_after();
             }
+            float f0 = 1.f, f1 = 0.f;  // of this tile's output and of its other half's
+            if (g.halves) {
+                if (t) {
+                    sh.half[r] = make_float2(m, z);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.half_full);
+                    if (!wait(&sh.half_empty, half_use++ & 1)) break;
+                    continue;
+                }
+                if (!wait(&sh.half_full, half_use++ & 1)) break;
+                tc_fence_after();
+                const float2 other = sh.half[r];
+                const float top = fmaxf(m, other.x), ref = top == -CUDART_INF_F ? 0.f : top;
+                f0 = z == 0.f ? 0.f : exp2f(m - ref);
+                f1 = other.y == 0.f ? 0.f : exp2f(other.x - ref);
+                z = z * f0 + other.y * f1;
+                m = top;
+            }
+            auto load_o = [&](uint32_t c, uint32_t (&o)[32]) {  // 32 channels of the row's output
+                if (!n) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0u;
+                    return;
+                }
+                tmem_ld32(o, o_addr + c);
+                tmem_wait_ld();
+                if (g.halves) {
+                    uint32_t x[32];
+                    tmem_ld32(x, o_addr + D + c);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + __uint_as_float(x[i]) * f1);
+                }
+            };
+            uint32_t again = 0;  // rows of this warp that are not finite though they see keys
+            const uint32_t warp_row = (warp & 3) * 32;
+            auto out_row = [&](uint32_t row) {
+                return reinterpret_cast<__nv_bfloat16*>(a.out) +
+                       ((uint64_t)(e.q0 + g.tok + row / a.group) * a.heads + head * a.group + row % a.group) * D;
+            };
             if (e.n_splits == 1) {
                 const float inv = 1.f / z;  // a row that sees no key: 0 * inf = NaN
                 float chk = 0.f;
-                __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) +
-                                     ((uint64_t)(e.q0 + token) * a.heads + head * a.group + hg) * D;
+                __nv_bfloat16* out = out_row(r);
 #pragma unroll
                 for (int c = 0; c < D; c += 32) {
                     uint32_t o[32];
-                    if (n) {
-                        tmem_ld32(o, o_addr + c);
-                        tmem_wait_ld();
-                    } else {
+                    load_o(c, o);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = 0u;
-                    }
+                    for (int i = 0; i < 32; i += 16) {
+                        uint32_t w[8];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        uint4 w;
-                        uint32_t* wp = &w.x;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
+                        for (int k = 0; k < 8; ++k) {
                             const float x = __uint_as_float(o[i + 2 * k]) * inv, y = __uint_as_float(o[i + 2 * k + 1]) * inv;
                             chk = fmaf(x, 0.f, chk);
                             chk = fmaf(y, 0.f, chk);
-                            wp[k] = pack_bf16x2(x, y);
+                            w[k] = pack_bf16x2(x, y);
                         }
-                        if (live) *reinterpret_cast<uint4*>(out + c + i) = w;
+                        if (live) {
+                            reinterpret_cast<uint4*>(out + c + i)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                            reinterpret_cast<uint4*>(out + c + i)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                        }
                     }
                 }
-                uint32_t again = __ballot_sync(0xffffffffu, live && lim > 0 && !(chk == 0.f));
-                if (again) {
-                    if (lane == 0) atomicAdd(&sh.redoing, 1);
-                    for (; again; again &= again - 1) {
-                        const int l = __ffs(again) - 1;
-                        redo_row<D>(a, e, head, __shfl_sync(0xffffffffu, token, l), __shfl_sync(0xffffffffu, hg, l));
-                    }
-                    __syncwarp();
-                    if (lane == 0) atomicSub(&sh.redoing, 1);
-                }
+                again = __ballot_sync(0xffffffffu, live && lim > 0 && !(chk == 0.f));
             } else {
                 // partial of this piece; the CTA that brings the last one merges them in the order of the pieces
                 auto slot_row = [&](uint32_t s, uint32_t row) {
                     return (uint64_t)((e.slot0 + s) * a.kv_heads + head) * a.l.slot_rows + t * kPromptTileRows + row;
                 };
                 const uint64_t at = slot_row(e.split, r);
-                if (n) {
 #pragma unroll
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(o, o_addr + c);
-                        tmem_wait_ld();
-                        if (live) {
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    load_o(c, o);
+                    if (live) {
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4)
-                                *reinterpret_cast<uint4*>(acc_ws + at * D + c + i) =
-                                    make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                        }
+                        for (int i = 0; i < 32; i += 8) st_global_v8(acc_ws + at * D + c + i, &o[i]);
                     }
                 }
                 if (live) *reinterpret_cast<float2*>(ml_ws + 2 * at) = make_float2(m, z);
@@ -562,54 +679,71 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (sh.last[t]) {
                     __threadfence();
                     if (r == 0) *cnt = 0;
-                    const uint32_t tok0 = g.tok;
-                    auto out_row = [&](uint32_t row) {
-                        return reinterpret_cast<__nv_bfloat16*>(a.out) +
-                               ((uint64_t)(e.q0 + tok0 + row / a.group) * a.heads + head * a.group + row % a.group) * D;
-                    };
-                    for (uint32_t i = r; i < live_rows * (D / 4); i += 128) {
-                        const uint32_t row = i / (D / 4), c = i % (D / 4) * 4;
-                        float top = -CUDART_INF_F, sum = 0.f;
-                        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                        for (uint32_t s = 0; s < e.n_splits; ++s)
-                            top = fmaxf(top, __ldcg(ml_ws + 2 * slot_row(s, row)));
-                        const float ref = top == -CUDART_INF_F ? 0.f : top;
-                        for (uint32_t s = 0; s < e.n_splits; ++s) {
-                            const uint64_t from = slot_row(s, row);
-                            const float2 mz = __ldcg(reinterpret_cast<const float2*>(ml_ws + 2 * from));
-                            if (mz.y == 0.f) continue;  // the row saw nothing of this piece
-                            const float f = exp2f(mz.x - ref);
-                            const float4 x = __ldcg(reinterpret_cast<const float4*>(acc_ws + from * D + c));
-                            sum += mz.y * f;
-                            o.x += x.x * f;
-                            o.y += x.y * f;
-                            o.z += x.z * f;
-                            o.w += x.w * f;
-                        }
-                        const float inv = 1.f / sum;
-                        o.x *= inv;
-                        o.y *= inv;
-                        o.z *= inv;
-                        o.w *= inv;
-                        *reinterpret_cast<uint2*>(out_row(row) + c) = make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
-                        if (!(o.x * 0.f + o.y * 0.f + o.z * 0.f + o.w * 0.f == 0.f)) sh.spoiled[t] = 1;
+                    // A warp merges its own 32 rows, all their loads of a piece in flight at once: lane l has
+                    // the weights of row l and 4 channels of every (D = 64: every other) row.
+                    constexpr int RPL = 128 / D;  // rows a load takes
+                    const uint32_t sub = lane / (D / 4), col = lane % (D / 4) * 4;
+                    float top = -CUDART_INF_F, sum = 0.f;
+                    if (live) {
+#pragma unroll 4
+                        for (uint32_t s = 0; s < e.n_splits; ++s) top = fmaxf(top, __ldcg(ml_ws + 2 * slot_row(s, r)));
                     }
-                    if (!meet()) break;
-                    if (*reinterpret_cast<volatile uint32_t*>(&sh.spoiled[t])) {
-                        if (lane == 0) atomicAdd(&sh.redoing, 1);
-                        for (uint32_t row = warp & 3; row < live_rows; row += 4) {
-                            const uint16_t* o = reinterpret_cast<const uint16_t*>(out_row(row));
-                            bool bad = false;
-                            for (uint32_t c = lane; c < D; c += 32) bad = bad || (o[c] & 0x7f80u) == 0x7f80u;
-                            if (__any_sync(0xffffffffu, bad)) redo_row<D>(a, e, head, tok0 + row / a.group, row % a.group);
+                    const float ref = top == -CUDART_INF_F ? 0.f : top;
+                    float4 o[32 / RPL];
+#pragma unroll
+                    for (int i = 0; i < 32 / RPL; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (uint32_t s = 0; s < e.n_splits; ++s) {
+                        float w = 0.f;
+                        if (live) {
+                            const float2 mz = __ldcg(reinterpret_cast<const float2*>(ml_ws + 2 * slot_row(s, r)));
+                            if (mz.y != 0.f) w = exp2f(mz.x - ref);  // 0: the row saw nothing of this piece
+                            sum += mz.y * w;
                         }
-                        __syncwarp();
-                        if (lane == 0) atomicSub(&sh.redoing, 1);
-                        if (!meet()) break;
-                        if (r == 0) sh.spoiled[t] = 0;
+                        const float* from = acc_ws + slot_row(s, warp_row) * D;
+#pragma unroll
+                        for (int i = 0; i < 32 / RPL; ++i) {
+                            const uint32_t row = i * RPL + sub;
+                            const float wr = __shfl_sync(0xffffffffu, w, row);
+                            if (warp_row + row < live_rows && wr != 0.f) {
+                                const float4 x = __ldcg(reinterpret_cast<const float4*>(from + row * D + col));
+                                o[i].x += x.x * wr;
+                                o[i].y += x.y * wr;
+                                o[i].z += x.z * wr;
+                                o[i].w += x.w * wr;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32 / RPL; ++i) {
+                        const uint32_t row = i * RPL + sub;
+                        const float inv = 1.f / __shfl_sync(0xffffffffu, sum, row);
+                        const float4 x = make_float4(o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv);
+                        const bool mine = warp_row + row < live_rows;
+                        if (mine)
+                            *reinterpret_cast<uint2*>(out_row(warp_row + row) + col) =
+                                make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+                        const uint32_t bad =
+                            __ballot_sync(0xffffffffu, mine && !(x.x * 0.f + x.y * 0.f + x.z * 0.f + x.w * 0.f == 0.f));
+#pragma unroll
+                        for (int k = 0; k < RPL; ++k)
+                            if (bad >> (k * (D / 4)) & (uint32_t)((1ull << (D / 4)) - 1)) again |= 1u << (i * RPL + k);
                     }
                 }
-                if (!meet()) break;  // sh.last and sh.spoiled have been read before the next item writes them
+                if (!meet()) break;  // sh.last has been read before the next item writes it
+            }
+            if (g.halves && lane == 0) {
+                tc_fence_before();
+                mbar_arrive(&sh.half_empty);  // O and the other half's have been read
+            }
+            if (again) {
+                if (lane == 0) atomicAdd(&sh.redoing, 1);
+                __syncwarp();
+                for (; again; again &= again - 1) {
+                    const uint32_t row = warp_row + __ffs(again) - 1;
+                    redo_row<D>(a, e, head, g.tok + row / a.group, row % a.group);
+                }
+                __syncwarp();
+                if (lane == 0) atomicSub(&sh.redoing, 1);
             }
             tc_fence_before();  // O has been read before the next item's first product may start (p_full)
         }
