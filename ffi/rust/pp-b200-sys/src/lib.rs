@@ -210,12 +210,10 @@ extern "C" {
                                  k_token_stride: u64, k_head_stride: u64, v_token_stride: u64, v_head_stride: u64,
                                  starts: *const u32, offsets: *const u32, status: *mut u32,
                                  stream: *mut c_void) -> i32;
-    pub fn pp_b200_token_logprobs_workspace_size(rows: u32, choices: u32, top: u32) -> usize;
     pub fn pp_b200_token_logprobs(logits: *const c_void, dtype: i32, rows: u32, choices: u32, row_stride: u64,
                                   targets: *const i32, bounds: *const u32, top: u32, logprob: *mut f32,
                                   entropy: *mut f32, rank: *mut u32, top_ids: *mut u32, top_logprobs: *mut f32,
-                                  workspace: *mut c_void, workspace_bytes: usize, status: *mut u32,
-                                  stream: *mut c_void) -> i32;
+                                  status: *mut u32, stream: *mut c_void) -> i32;
     pub fn pp_b200_prepare(device: i32) -> i32;
     pub fn pp_b200_prepare_optional(device: i32, fusion: u32, split_k: u32, model_dtype: i32, head_width: u32,
                                     ffn_hidden: u32) -> i32;

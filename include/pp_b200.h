@@ -300,9 +300,6 @@ int32_t pp_b200_prompt_append(const PpKvArena* arena, const void* k, const void*
                               uint64_t v_head_stride, const uint32_t* starts, const uint32_t* offsets,
                               uint32_t* status, void* stream);
 
-/* Workspace bytes of pp_b200_token_logprobs (0 when it needs none). */
-size_t pp_b200_token_logprobs_workspace_size(uint32_t rows, uint32_t choices, uint32_t top);
-
 /* Log probabilities of given tokens with entropy and the best alternatives,
  * over the head outputs the sampler reads.
  *   logits    f32/bf16 [rows, choices], row stride row_stride elements
@@ -327,8 +324,7 @@ size_t pp_b200_token_logprobs_workspace_size(uint32_t rows, uint32_t choices, ui
 int32_t pp_b200_token_logprobs(const void* logits, int32_t dtype, uint32_t rows, uint32_t choices,
                                uint64_t row_stride, const int32_t* targets, const uint32_t* bounds, uint32_t top,
                                float* logprob, float* entropy, uint32_t* rank, uint32_t* top_ids,
-                               float* top_logprobs, void* workspace, size_t workspace_bytes, uint32_t* status,
-                               void* stream);
+                               float* top_logprobs, uint32_t* status, void* stream);
 
 /* Diagnostic: runs one bounded wait on a barrier that nothing completes, with
  * the library's wait loop and a limit of limit_us microseconds (1..10^6), so a

@@ -62,7 +62,6 @@ EXPORTED = (
     "pp_b200_plan_prompt",
     "pp_b200_prompt_attention",
     "pp_b200_prompt_append",
-    "pp_b200_token_logprobs_workspace_size",
     "pp_b200_token_logprobs",
     "pp_b200_prepare",
     "pp_b200_prepare_optional",
@@ -201,8 +200,7 @@ def _load() -> C.CDLL:
         "pp_b200_plan_prompt": (i32, [P(PpPrompt), vp, vp, vp, sz, vp, vp]),
         "pp_b200_prompt_attention": (i32, [P(PpPrompt), vp, vp, vp, vp, sz, vp, vp]),
         "pp_b200_prompt_append": (i32, [P(PpKvArena), vp, vp, i32, u32, u64, u64, u64, u64, vp, vp, vp, vp]),
-        "pp_b200_token_logprobs_workspace_size": (sz, [u32, u32, u32]),
-        "pp_b200_token_logprobs": (i32, [vp, i32, u32, u32, u64, vp, vp, u32, vp, vp, vp, vp, vp, vp, sz, vp, vp]),
+        "pp_b200_token_logprobs": (i32, [vp, i32, u32, u32, u64, vp, vp, u32, vp, vp, vp, vp, vp, vp, vp]),
         "pp_b200_prepare": (i32, [i32]),
         "pp_b200_prepare_optional": (i32, [i32, u32, u32, i32, u32, u32]),
     }

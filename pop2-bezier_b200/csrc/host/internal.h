@@ -234,7 +234,6 @@ struct LogprobsLaunch {
     uint32_t* rank;
     uint32_t* top_ids;
     float* top_logprobs;
-    unsigned char* ws;
     uint32_t* status;
     uint32_t num_sms;
 };

@@ -177,13 +177,10 @@ int32_t pp_b200_prompt_append(const PpKvArena* arena, const void* k, const void*
     return pp::cuda_status(pp::launch_prompt_append(P, (cudaStream_t)stream), "prompt append launch");
 }
 
-size_t pp_b200_token_logprobs_workspace_size(uint32_t, uint32_t, uint32_t) { return 0; }
-
 int32_t pp_b200_token_logprobs(const void* logits, int32_t dtype, uint32_t rows, uint32_t choices,
                                uint64_t row_stride, const int32_t* targets, const uint32_t* bounds, uint32_t top,
                                float* logprob, float* entropy, uint32_t* rank, uint32_t* top_ids,
-                               float* top_logprobs, void* workspace, size_t workspace_bytes, uint32_t* status,
-                               void* stream) {
+                               float* top_logprobs, uint32_t* status, void* stream) {
     if (dtype != PP_DTYPE_F32 && dtype != PP_DTYPE_BF16)
         return fail_fmt(PP_STATUS_PRECONDITION, "token logprobs: unsupported dtype %d", dtype);
     if (choices == 0 || choices > 0x7fffffffu || rows > 0x7fffffffu || top > 32)
@@ -202,9 +199,6 @@ int32_t pp_b200_token_logprobs(const void* logits, int32_t dtype, uint32_t rows,
         !aligned(logprob, 4) || !aligned(entropy, 4) || !aligned(rank, 4) || !aligned(top_ids, 4) ||
         !aligned(top_logprobs, 4) || !aligned(status, 4))
         return fail_fmt(PP_STATUS_PRECONDITION, "token logprobs: misaligned pointer");
-    const size_t need = pp_b200_token_logprobs_workspace_size(rows, choices, top);
-    if (need && (!workspace || !aligned(workspace, 256) || workspace_bytes < need))
-        return fail_fmt(PP_STATUS_PRECONDITION, "token logprobs: workspace of %zu bytes, 256-byte aligned, needed", need);
     L.logits = logits;
     L.bf16 = dtype == PP_DTYPE_BF16;
     L.rows = rows;
@@ -218,7 +212,6 @@ int32_t pp_b200_token_logprobs(const void* logits, int32_t dtype, uint32_t rows,
     L.rank = rank;
     L.top_ids = top_ids;
     L.top_logprobs = top_logprobs;
-    L.ws = static_cast<unsigned char*>(workspace);
     L.status = status;
     return pp::cuda_status(pp::launch_token_logprobs(L, (cudaStream_t)stream), "token logprobs launch");
 }

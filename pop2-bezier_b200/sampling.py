@@ -55,7 +55,7 @@ class TokenLogprobs(NamedTuple):
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0, bounds: torch.Tensor | None = None,
-                   workspace: torch.Tensor | None = None, status: torch.Tensor | None = None) -> TokenLogprobs:
+                   status: torch.Tensor | None = None) -> TokenLogprobs:
     """Scores targets (int32 [rows], columns of their rows; -1: none) under
     logits f32/bf16 [rows, choices] (any row stride): log probability, rank,
     entropy and the `top` (at most 32) best alternatives.
@@ -68,7 +68,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0,
     one outside the choices, which also sets DEV_WINDOW_RANGE in the status
     word.  NaN or +inf in the window makes log probabilities and entropy NaN.
     """
-    ops._require_cuda(logits, targets, bounds, workspace, status)
+    ops._require_cuda(logits, targets, bounds, status)
     if logits.dim() != 2 or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise N.PreconditionError("token logprobs need logits [rows, choices] with contiguous rows and a nonempty head")
     rows, choices = logits.shape
@@ -87,11 +87,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0,
     ids = torch.empty((rows, top), dtype=torch.int32, device=dev) if top else None
     best = torch.empty((rows, top), dtype=torch.float32, device=dev) if top else None
     with torch.cuda.device(dev):
-        if workspace is None:
-            need = N.lib.pp_b200_token_logprobs_workspace_size(rows, choices, top)
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         N.check(N.lib.pp_b200_token_logprobs(
             logits.data_ptr(), code, rows, choices, stride, targets.data_ptr(), ops._ptr(bounds), top,
-            logprob.data_ptr(), entropy.data_ptr(), rank.data_ptr(), ops._ptr(ids), ops._ptr(best), ops._ptr(workspace),
-            workspace.numel() if workspace is not None else 0, ops._ptr(status), ops._stream(logits)))
+            logprob.data_ptr(), entropy.data_ptr(), rank.data_ptr(), ops._ptr(ids), ops._ptr(best),
+            ops._ptr(status), ops._stream(logits)))
     return TokenLogprobs(logprob, entropy, rank, ids, best)

@@ -8,7 +8,10 @@ threads, warps and pieces), and the sum has n terms added in chains of at most
 n / 32 + 64.  So s is off by at most
   r = 41 * 2^-21 + 2^-22 a + (n / 32 + 64) 2^-24       relatively,
 a = sum e_i |x_i - m| / s, which moves log1p(s) by at most r s / (1 + s) and
-d / (1 + s) by 2 r times itself.  The result is rounded to f32 (2^-24)."""
+d / (1 + s) by 2 r times itself.  The result is rounded to f32 (2^-24).  An e_i
+below 2^-126, the least normal f32, may count as 0: n of them move s, and so
+log1p(s), by less than n 2^-126, and d, with |x_i - m| < 2^8 where e_i >= 2^-300
+and nothing to speak of below, by less than n 2^-118."""
 from __future__ import annotations
 
 import math
@@ -37,7 +40,7 @@ def exact(x, targets, bounds, top):
     tail = torch.log1p(s)[:, None]
     ent = tail[:, 0] + d / (1 + s)
     r = 41 * 2.0**-21 + 2.0**-22 * (d / s.clamp(min=1e-300)) + (c / 32 + 64) * 2.0**-24
-    err_lse = r * s / (1 + s)
+    err_lse = r * s / (1 + s) + c * 2.0**-126
     t = targets.long()[:, None]
     ok = (t >= lo) & (t < hi)
     tc = t.clamp(0, c - 1)
@@ -52,7 +55,7 @@ def exact(x, targets, bounds, top):
     ids[:, :k] = torch.where(listed, order.indices[:, :k], -1)
     best[:, :k] = torch.where(listed, order.values[:, :k] - m - tail, -math.inf)
     return dict(lp=lp, ent=ent, rank=rank, ids=ids, best=best, err_lse=err_lse,
-                err_ent=err_lse + 2 * r * d / (1 + s))
+                err_ent=err_lse + 2 * r * d / (1 + s) + c * 2.0**-118)
 
 
 def near(got, want, err):

@@ -100,7 +100,7 @@ def test_append_arena(pp):
 def test_logprobs(pp, bad):
     N = pp._native
     a = dict(logits=4096, dtype=0, rows=4, choices=100, stride=100, targets=64, bounds=None, top=2, lp=64, ent=64,
-             rank=64, ids=64, best=64, ws=None, ws_bytes=0, status=None, stream=None)
+             rank=64, ids=64, best=64, status=None, stream=None)
     a.update(bad)
     assert N.lib.pp_b200_token_logprobs(*a.values()) == N.STATUS_PRECONDITION
     assert "token logprobs" in N.last_error()
