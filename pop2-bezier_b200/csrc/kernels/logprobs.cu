@@ -10,19 +10,24 @@
 // of x = m.  When the maximum rises by g, both change by exp(-g), and d by
 // (d + g (s + count)) exp(-g).
 //
-// A lane holds 8 vectors of 16 bytes in registers: they are read once and looked
-// at several times (maximum, sums, rank, alternatives).  NW warps take 4 KB each
-// of a row; a longer row is taken in steps, or by a cluster of up to 8 CTAs
-// that merge through their shared memory, when there are few rows.
+// A thread copies 8 vectors of 16 bytes into shared memory (cp.async) and looks at
+// them several times (maximum, sums, rank, alternatives) in short loops, while its
+// next 8 are on their way: nothing waits for another thread's copies, and the
+// loops stay in the instruction cache, which the same code unrolled over
+// registers did not (4096 rows of 32768: 154 us).  NW warps take 4 KB each of a
+// row; a longer row is taken in steps, with one barrier each, or by a cluster of
+// up to 8 CTAs that merge through their shared memory, when there are few rows.
 //
-// Alternatives: the k-th largest of a warp's 32 lane maxima is no larger than
-// the k-th largest logit, and neither is the largest such bound of all warps.
-// Only logits from that bound on are candidates, on random rows about k of
-// them; one warp sorts them 32 at a time and keeps the best 32 as a sorted list,
-// one a lane.  Where the bound leaves more than the buffer holds (long ties),
-// the block takes the maximum k times instead.
+// Alternatives: with q = ceil(k / NW), the q-th largest lane maximum of ceil(k / q)
+// warps is reached by at least k logits, so the least of these is no larger than
+// the k-th best.  Only logits from the best such bound on are candidates (on
+// random rows a few times k of them); they wait in a buffer a warp until the row
+// ends or a buffer is half full.  A candidate's place in the list is the number
+// of candidates ahead of it, which one thread each counts.  Where a step leaves
+// more candidates than a buffer holds (long ties), the block takes the maximum k
+// times instead.
 //
-// Bound by HBM on long rows; issue slots come next (about 9 a bf16 element).
+// Bound by HBM on long rows; issue slots and the latency of a step come next.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -31,11 +36,9 @@
 namespace pp {
 namespace {
 
-#ifndef LOGPROBS_WARPS
-#define LOGPROBS_WARPS 32  // resident warps of an SM: bounds the registers
-#endif
 constexpr int kVecs = 8;              // 16-byte vectors a lane holds
-constexpr uint32_t kCandidates = 512;
+constexpr uint32_t kCandidates = 64;  // of a warp
+constexpr int kMostWarps = 8;          // of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
@@ -109,18 +112,6 @@ __device__ __forceinline__ T sort32(T x, uint32_t lane) {
     return x;
 }
 
-// The best 32 of two sorted lists, sorted.
-__device__ __forceinline__ unsigned long long merge32(unsigned long long a, unsigned long long b, uint32_t lane) {
-    b = __shfl_sync(0xffffffffu, b, 31 - lane);
-    unsigned long long x = a > b ? a : b;
-#pragma unroll
-    for (uint32_t j = 16; j; j >>= 1) {
-        const unsigned long long y = __shfl_xor_sync(0xffffffffu, x, j);
-        x = ((lane & j) == 0) == (x > y) ? x : y;
-    }
-    return x;
-}
-
 template <bool BF>
 __device__ __forceinline__ float load_logit(const void* p, uint64_t i) {
     if constexpr (BF) return bf16_lo_to_f32(__ldg(reinterpret_cast<const unsigned short*>(p) + i));
@@ -138,6 +129,27 @@ __device__ __forceinline__ float element(const uint4& v, int i) {
 __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// Element i of a vector in shared memory, i not known beforehand.
+template <bool BF>
+__device__ __forceinline__ float picked(const uint4* p, int i) {
+    if constexpr (BF) return bf16_lo_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
+    else return reinterpret_cast<const float*>(p)[i];
+}
+
+// 1 in each half where a > b (ge: a >= b), as bf16; NaN gives 0.
+template <bool GE>
+__device__ __forceinline__ uint32_t above_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (GE) asm("set.ge.bf16x2.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("set.gt.bf16x2.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 
@@ -166,115 +178,187 @@ __device__ __forceinline__ uint32_t ld_peer(const void* p, uint32_t rank) {
     return v;
 }
 
+// Floats of shared memory that only rise, as integers in their order.
+__device__ __forceinline__ int rising(float x) {
+    const int b = __float_as_int(x);
+    return b ^ (b >> 31 & 0x7fffffff);
+}
+__device__ __forceinline__ float rising_value(int k) { return __int_as_float(k ^ (k >> 31 & 0x7fffffff)); }
+
+__device__ __forceinline__ void copy16(uint4* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_sent() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LATER>
+__device__ __forceinline__ void copies_landed() {  // all but the last LATER groups
+    asm volatile("cp.async.wait_group %0;" ::"n"(LATER) : "memory");
+}
+
+// The list of the best 32 from the candidates and the list before it, by all of the block.
+__device__ __noinline__ void sort_candidates(const unsigned long long* cand, uint32_t count,
+                                             const unsigned long long* old, unsigned long long* list, uint32_t k) {
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t before = __popc(__ballot_sync(0xffffffffu, lane < k && old[lane] != 0ull));
+    if (threadIdx.x < 32 && lane >= count + before) list[lane] = 0ull;
+    for (uint32_t j = threadIdx.x; j < count + before; j += blockDim.x) {
+        const unsigned long long mine = j < count ? cand[j] : old[j - count];
+        uint32_t place = 0;
+#pragma unroll 4
+        for (uint32_t i = 0; i < count; ++i) place += cand[i] > mine;
+#pragma unroll 4
+        for (uint32_t i = 0; i < before; ++i) place += old[i] > mine;
+        if (place < 32) list[place] = mine;
+    }
+}
+
 template <bool BF, int NW>
-__global__ void __launch_bounds__(32 * NW, LOGPROBS_WARPS / NW) logprobs_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
     constexpr int EPV = BF ? 8 : 4;                    // elements of a vector
-    constexpr uint32_t STEP = NW * 32 * kVecs;         // vectors a CTA holds
-    __shared__ float s_max[NW], s_bound[NW], s_kth;
-    __shared__ unsigned long long s_cand[kCandidates], s_list[32], s_best[NW];
-    __shared__ uint32_t s_count[2];
+    constexpr uint32_t T = 32 * NW, STEP = T * kVecs;  // vectors a CTA takes at a time
+    constexpr int kLow = (int)0x807fffff;              // rising(-inf)
+    extern __shared__ uint4 s_row[];                   // one or two steps, vector v of thread t at v T + t
+    __shared__ int s_top[2][NW], s_reached[2][NW];
+    __shared__ unsigned long long s_cand[NW * kCandidates], s_list[2][32], s_best[NW];
+    __shared__ uint32_t s_count;
     __shared__ Part s_part[NW], s_cta;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t row = blockIdx.x / a.cluster, part = a.cluster > 1 ? cluster_rank() : 0u;
+    const uint32_t row = a.cluster > 1 ? blockIdx.x / a.cluster : blockIdx.x, part = a.cluster > 1 ? cluster_rank() : 0u;
     const uint32_t k = a.top;
+    if (threadIdx.x == 0) s_count = 0;
+    if (warp == 0) s_list[0][lane] = 0ull;
+    const uint32_t q = (k + NW - 1) / NW;  // lane maxima of a warp that have to reach the bound
+    const uint32_t bounding = k ? (k + q - 1) / q : 0u;
     pdl_wait_primary();
     const uint64_t base = (uint64_t)row * a.stride;
-    uint32_t lo = 0, n = a.choices;
+    int lo = 0, n = (int)a.choices;  // columns are below 2^31
     if (a.bounds) {
-        lo = a.bounds[2 * row];
-        n = a.bounds[2 * row + 1];
-        if ((uint64_t)lo + n > a.choices) {
-            if (threadIdx.x == 0 && part == 0 && a.status) atomicOr(a.status, PP_DEV_WINDOW_RANGE);
-            lo = n = 0;
-        }
+        const uint32_t from = a.bounds[2 * row], count = a.bounds[2 * row + 1];
+        const bool fits = (uint64_t)from + count <= a.choices;
+        if (!fits && threadIdx.x == 0 && part == 0 && a.status) atomicOr(a.status, PP_DEV_WINDOW_RANGE);
+        lo = fits ? (int)from : 0;
+        n = fits ? (int)count : 0;
     }
-    const uint32_t hi = lo + n;
-    const int64_t target = a.targets[row];
-    const bool inside = target >= lo && target < (int64_t)hi;
-    const uint32_t t = inside ? (uint32_t)target : 0u;
-    const float xt = inside ? load_logit<BF>(a.logits, base + t) : -CUDART_INF_F;
-    // ahead of the target: x > xt behind it, x >= xt (x > the float below xt) before it.  A NaN or -inf target is
-    // counted by itself, below.
-    const bool ordinary = inside && xt > -CUDART_INF_F;
-    const float below = ordinary ? nextafterf(xt, -CUDART_INF_F) : 0.f;
-
+    const int hi = lo + n;
     // Vectors lie on 16-byte boundaries of memory: vector v holds the columns first + v * EPV ...
-    const uint64_t addr = reinterpret_cast<uint64_t>(a.logits) + (base + lo) * (BF ? 2 : 4);
-    const int64_t first = (int64_t)lo - (int64_t)(addr % 16 / (BF ? 2 : 4));
-    const uint32_t vectors = n ? (uint32_t)((hi - first + EPV - 1) / EPV) : 0u;
+    const char* row_ptr = reinterpret_cast<const char*>(a.logits) + base * (BF ? 2 : 4);
+    const int first = lo - (int)((reinterpret_cast<uint64_t>(row_ptr) + (uint64_t)lo * (BF ? 2 : 4)) % 16 / (BF ? 2 : 4));
+    const uint32_t vectors = n ? ((uint32_t)(hi - first) + EPV - 1) / EPV : 0u;
 
-    Part p{-CUDART_INF_F, 0.f, 0.f, 0.f, 0u};
-    unsigned long long list = 0;  // warp 0: the best so far, sorted over the lanes
-    if (threadIdx.x == 0) {
-        s_count[0] = 0;
-        s_kth = -CUDART_INF_F;
-    }
-    uint32_t turn = 0;  // the two counts take turns: one is emptied when nobody reads it
-    for (uint64_t v0 = (uint64_t)part * STEP; v0 < vectors; v0 += (uint64_t)a.cluster * STEP, turn ^= 1) {
-        uint4 x[kVecs];
-        float vm[kVecs];
-        const uint32_t mine = (uint32_t)v0 + warp * 32 * kVecs + lane;
-#pragma unroll
+    auto fetch = [&](uint32_t v0, uint4* to) {
+#pragma unroll 4
         for (int v = 0; v < kVecs; ++v) {
-            const uint32_t at = mine + 32 * v;
-            const int64_t col = first + (int64_t)at * EPV;
-            const uint32_t none = BF ? 0xff80ff80u : 0xff800000u;  // -inf
-            x[v] = make_uint4(none, none, none, none);
-            if (at < vectors) {
-                if (col >= lo && col + EPV <= hi) {
-                    if constexpr (BF)
-                        x[v] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.logits) + base + col));
-                    else x[v] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(a.logits) + base + col));
-                } else {  // an end of the window
-                    uint32_t w[4] = {none, none, none, none};
-#pragma unroll
+            const uint32_t at = v0 + v * T + threadIdx.x;
+            const int col = first + (int)at * EPV;
+            if (at < vectors && col >= lo && col + EPV <= hi) {
+                copy16(to + v * T + threadIdx.x, row_ptr + (int64_t)col * (BF ? 2 : 4));
+            } else {  // an end of the window, or nothing
+                const uint32_t none = BF ? 0xff80ff80u : 0xff800000u;  // -inf
+                uint4 y = make_uint4(none, none, none, none);
+                to[v * T + threadIdx.x] = y;
+                if (at < vectors) {
                     for (int i = 0; i < EPV; ++i)
                         if (col + i >= lo && col + i < hi) {
                             const uint32_t bits = __float_as_uint(load_logit<BF>(a.logits, base + col + i));
-                            if constexpr (BF) w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | bits : (w[i / 2] & 0xffff0000u) | bits >> 16;
-                            else w[i] = bits;
+                            if constexpr (BF)
+                                reinterpret_cast<uint16_t*>(to + v * T + threadIdx.x)[i] = (uint16_t)(bits >> 16);
+                            else reinterpret_cast<uint32_t*>(to + v * T + threadIdx.x)[i] = bits;
                         }
-                    x[v] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
         }
-        float top = -CUDART_INF_F;
-#pragma unroll
-        for (int v = 0; v < kVecs; ++v) {
-            vm[v] = vector_max<BF>(x[v]);
-            top = fmaxf(top, vm[v]);
-        }
-        float bound = -CUDART_INF_F;
-        if (k) {
-            top = sort32(top, lane);
-            bound = __shfl_sync(0xffffffffu, top, k - 1);
+        copies_sent();
+    };
+    const uint32_t stride = a.cluster * STEP;
+    uint4* now = s_row;
+    uint4* later = s_row + STEP;
+    if (part * STEP < vectors) fetch(part * STEP, now);
+
+    const int t = a.targets[row];
+    const bool inside = t >= lo && t < hi;
+    const float xt = inside ? load_logit<BF>(a.logits, base + t) : -CUDART_INF_F;
+    // ahead of the target: x > xt behind it, x >= xt before it.  A NaN or -inf target is counted by itself, below.
+    const bool ordinary = inside && xt > -CUDART_INF_F;
+
+    Part p{-CUDART_INF_F, 0.f, 0.f, 0.f, 0u};
+    uint32_t turn = 0;     // steps take turns at what the warps tell each other
+    uint32_t current = 0;  // which of the two lists is the last one
+    uint32_t found = 0;    // candidates of the warp
+    float bound = -CUDART_INF_F;
+    bool over = false;  // candidates did not fit: the list is found in the row again
+    __syncthreads();
+    for (uint32_t v0 = part * STEP; v0 < vectors; v0 += stride, turn ^= 1) {
+        if (v0 + stride < vectors) {
+            fetch(v0 + stride, later);
+            copies_landed<1>();
         } else {
-#pragma unroll
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            copies_landed<0>();
         }
-        if (lane == 0) {
-            s_max[warp] = top;
-            s_bound[warp] = bound;
+        const uint4* x = now + threadIdx.x;
+        float top = -CUDART_INF_F;
+#pragma unroll 4
+        for (int v = 0; v < kVecs; ++v) top = fmaxf(top, vector_max<BF>(x[v * T]));
+        const int key = rising(top);
+        const int warp_key = __reduce_max_sync(0xffffffffu, key);
+        const float warp_top = rising_value(warp_key);
+        if (k) {
+            int reached = warp_key;
+            if (q > 8) {
+                reached = __shfl_sync(0xffffffffu, sort32(key, lane), q - 1);
+            } else {
+                uint32_t left = 0xffffffffu;  // lanes not taken yet
+                for (uint32_t i = 1; i < q; ++i) {
+                    const uint32_t best = __ballot_sync(0xffffffffu, (left >> lane & 1u) && key == reached);
+                    left &= ~(best & (0u - best));
+                    reached = __reduce_max_sync(0xffffffffu, left >> lane & 1u ? key : kLow);
+                }
+            }
+            if (lane == 0) s_reached[turn][warp] = reached;
         }
-        __syncthreads();
+        if (lane == 0) s_top[turn][warp] = warp_key;
+        if (__syncthreads_or(found > kCandidates / 2)) {  // a warp has used half its share of the buffer
+            over = __syncthreads_or(found > kCandidates) || over;
+            if (!over) sort_candidates(s_cand, s_count, s_list[current], s_list[current ^ 1], k);
+            __syncthreads();
+            if (threadIdx.x == 0) s_count = 0;
+            found = 0;
+            current ^= 1;
+            const unsigned long long kth = s_list[current][k - 1];
+            if (!over && kth) bound = fmaxf(bound, order_value(kth));
+            __syncthreads();
+        }
         float m = p.m;
-        bound = s_kth;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            m = fmaxf(m, s_max[w]);
-            bound = fmaxf(bound, s_bound[w]);
+        for (int w = 0; w < NW; ++w) m = fmaxf(m, rising_value(s_top[turn][w]));
+        if (k) {
+            int reached = 0x7fffffff;
+#pragma unroll
+            for (int w = 0; w < NW; ++w)
+                if (w < bounding) reached = min(reached, s_reached[turn][w]);
+            bound = fmaxf(bound, rising_value(reached));
         }
         raise(p, m);
+        // y = x log2(e) - r with r = m log2(e) rounded: all e come out 2^slip too large, which is taken back below
         const float ref = m > -CUDART_INF_F ? m : 0.f;  // nothing but -inf so far (or NaN, which has to show in s)
-        const uint64_t neg = f2_pack(-ref, -ref), l2e = f2_pack(kLog2e, kLog2e);
+        const float r = ref * kLog2e, slip = fmaf(ref, kLog2e, -r);
+        const uint64_t neg = f2_pack(-r, -r), l2e = f2_pack(kLog2e, kLog2e);
         uint64_t s0 = 0ull, s1 = 0ull, d0 = 0ull, d1 = 0ull;
-#pragma unroll
+        uint32_t ahead2 = 0;  // two bf16 counts, at most 32 each
+        const bool look = ordinary && warp_top >= xt;
+        // No x is taken below `low`, at least 119 under the maximum also as bf16: exp2 of its y is 0, and so is their
+        // product, which that of -inf would not be.  Beyond 2^20 the slip is no small number: one by one then.
+        const float low = ref - 120.f - 0.01f * fabsf(ref);
+        const bool plain = fabsf(ref) < 1048576.f;
+        const uint32_t low2 = pack_bf16x2(low, low), xt2 = pack_bf16x2(xt, xt);
+#pragma unroll 2
         for (int v = 0; v < kVecs; ++v) {
-            const int64_t col = first + (int64_t)(mine + 32 * v) * EPV;
-            if (vm[v] == m) {  // holds the maximum: it is counted, not summed
-#pragma unroll
+            const uint4 y4 = x[v * T];
+            const uint32_t w[4] = {y4.x, y4.y, y4.z, y4.w};
+            const float vm = vector_max<BF>(y4);
+            const int col = first + (int)(v0 + v * T + threadIdx.x) * EPV;
+            if (vm == m || !plain) {  // holds the maximum: it is counted, not summed
+#pragma unroll 1
                 for (int i = 0; i < EPV; ++i) {
-                    const float e = element<BF>(x[v], i);
+                    const float e = picked<BF>(x + v * T, i);
                     const float y = fmaxf((e - ref) * kLog2e, -160.f), f = e == m ? 0.f : fast_exp2(e == e ? y : e);
                     p.c += e == m ? 1.f : 0.f;
                     p.s += f;
@@ -283,93 +367,121 @@ __global__ void __launch_bounds__(32 * NW, LOGPROBS_WARPS / NW) logprobs_kernel(
             } else {
 #pragma unroll
                 for (int i = 0; i < EPV; i += 2) {
-                    float y0, y1;
-                    f2_unpack(f2_mul(f2_add(f2_pack(element<BF>(x[v], i), element<BF>(x[v], i + 1)), neg), l2e), y0, y1);
-                    // exp2(-160) is 0 and so is its product with y, which -inf would make NaN
-                    asm("max.NaN.f32 %0, %0, %1;" : "+f"(y0) : "f"(-160.f));
-                    asm("max.NaN.f32 %0, %0, %1;" : "+f"(y1) : "f"(-160.f));
+                    float x0, x1, y0, y1;
+                    if constexpr (BF) {
+                        uint32_t u;
+                        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(u) : "r"(w[i / 2]), "r"(low2));
+                        x0 = bf16_lo_to_f32(u);
+                        x1 = bf16_hi_to_f32(u);
+                    } else {
+                        asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(__uint_as_float(w[i])), "f"(low));
+                        asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(__uint_as_float(w[i + 1])), "f"(low));
+                    }
+                    uint64_t y2;
+                    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y2) : "l"(f2_pack(x0, x1)), "l"(l2e), "l"(neg));
+                    f2_unpack(y2, y0, y1);
                     const uint64_t e2 = f2_pack(fast_exp2(y0), fast_exp2(y1));
                     uint64_t& s = i & 2 ? s1 : s0;
                     uint64_t& d = i & 2 ? d1 : d0;
                     s = f2_add(s, e2);
-                    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(e2), "l"(f2_pack(y0, y1)));
+                    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(e2), "l"(y2));
                 }
             }
-            if (ordinary && vm[v] >= xt) {
-                const float edge = col < t ? below : xt;
+            if (look && vm >= xt) {
                 if (col <= t && t < col + EPV) {
+#pragma unroll 1
+                    for (int i = 0; i < EPV; ++i) {
+                        const float e = picked<BF>(x + v * T, i);
+                        p.ahead += e > xt || (e == xt && col + i < t);
+                    }
+                } else if constexpr (BF) {
+                    // x >= xt is x > the bf16 below xt, but not at the ends of the type: two loops
+                    if (col < t) {
 #pragma unroll
-                    for (int i = 0; i < EPV; ++i) p.ahead += element<BF>(x[v], i) > (col + i < t ? below : xt);
+                        for (int i = 0; i < 4; ++i) ahead2 = add_bf16x2(ahead2, above_bf16x2<true>(w[i], xt2));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) ahead2 = add_bf16x2(ahead2, above_bf16x2<false>(w[i], xt2));
+                    }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < EPV; ++i) p.ahead += element<BF>(x[v], i) > edge;
-                }
-            }
-            if (k && vm[v] >= bound) {
-#pragma unroll
-                for (int i = 0; i < EPV; ++i) {
-                    const float e = element<BF>(x[v], i);
-                    if (e >= bound && e > -CUDART_INF_F) {
-                        const uint32_t at = atomicAdd(&s_count[turn], 1u);
-                        if (at < kCandidates) s_cand[at] = order_of(e, (uint32_t)col + i);
+                    for (int i = 0; i < EPV; ++i) {
+                        const float e = __uint_as_float(w[i]);
+                        p.ahead += col < t ? e >= xt : e > xt;
                     }
                 }
             }
-            asm volatile("" ::: "memory");  // one vector at a time: unpacked, they would not fit the registers
-        }
-        float e0, e1, e2, e3;
-        f2_unpack(f2_add(s0, s1), e0, e1);
-        f2_unpack(f2_add(d0, d1), e2, e3);
-        p.s += e0 + e1;
-        p.d -= (e2 + e3) * 0.6931471805599453f;
-        if (k) {
-            __syncthreads();
-            const uint32_t count = s_count[turn];
-            if (count <= kCandidates) {
-                if (warp == 0) {
-                    for (uint32_t c = 0; c < count; c += 32)
-                        list = merge32(list, sort32(c + lane < count ? s_cand[c + lane] : 0ull, lane), lane);
+            if (k && __any_sync(0xffffffffu, vm >= bound && vm > -CUDART_INF_F)) {
+                uint32_t have = 0;  // candidates of the lane's vector, as bits
+#pragma unroll
+                for (int i = 0; i < EPV; ++i) {
+                    const float e = element<BF>(y4, i);
+                    have |= (e >= bound && e > -CUDART_INF_F ? 1u : 0u) << i;
                 }
-            } else {
-                const int64_t from = max((int64_t)lo, first + (int64_t)v0 * EPV);
-                const int64_t to = min((int64_t)hi, first + (int64_t)(v0 + STEP) * EPV);
-                unsigned long long prev = ~0ull, found = 0;
-                for (uint32_t j = 0; j < k; ++j) {
-                    unsigned long long best = 0;
-                    for (int64_t i = from + threadIdx.x; i < to; i += 32 * NW) {
+                for (uint32_t who; (who = __ballot_sync(0xffffffffu, have != 0)) != 0; have &= have - 1) {
+                    uint32_t at = 0;
+                    found += __popc(who);
+                    if (lane == 0 && found <= kCandidates) at = atomicAdd(&s_count, __popc(who));
+                    at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+                    if (have && found <= kCandidates) {
+                        const int i = __ffs(have) - 1;
+                        s_cand[at] = order_of(picked<BF>(x + v * T, i), (uint32_t)(col + i));
+                    }
+                }
+            }
+        }
+        if constexpr (BF) p.ahead += (uint32_t)(bf16_lo_to_f32(ahead2) + bf16_hi_to_f32(ahead2));
+        if (plain) {
+            float e0, e1, e2, e3;
+            f2_unpack(f2_add(s0, s1), e0, e1);
+            f2_unpack(f2_add(d0, d1), e2, e3);
+            const float sum = e0 + e1, back = fast_exp2(-slip);
+            p.s += sum * back;
+            p.d -= (e2 + e3 - slip * sum) * back * 0.6931471805599453f;
+        }
+        uint4* done = now;
+        now = later;
+        later = done;
+    }
+    if (k) {
+        over = __syncthreads_or(found > kCandidates) || over;
+        if (!over) {
+            sort_candidates(s_cand, s_count, s_list[current], s_list[current ^ 1], k);
+            current ^= 1;
+        } else {
+            unsigned long long* list = s_list[current];
+            __syncthreads();
+            unsigned long long prev = ~0ull;
+            for (uint32_t j = 0; j < k; ++j) {
+                unsigned long long best = 0;
+                for (uint32_t v0 = part * STEP; v0 < vectors; v0 += stride) {
+                    const int64_t from = max((int64_t)lo, first + (int64_t)v0 * EPV);
+                    const int64_t to = min((int64_t)hi, first + ((int64_t)v0 + STEP) * EPV);
+                    for (int64_t i = from + threadIdx.x; i < to; i += T) {
                         const float e = load_logit<BF>(a.logits, base + i);
-                        if (!(e >= bound && e > -CUDART_INF_F)) continue;
+                        if (!(e > -CUDART_INF_F)) continue;
                         const unsigned long long o = order_of(e, (uint32_t)i);
                         if (o < prev && o > best) best = o;
                     }
+                }
 #pragma unroll
-                    for (int o = 16; o; o >>= 1) {
-                        const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, o);
-                        best = best > y ? best : y;
-                    }
-                    if (lane == 0) s_best[warp] = best;
-                    __syncthreads();
-                    for (int w = 0; w < NW; ++w) best = best > s_best[w] ? best : s_best[w];
-                    if (lane == j) found = best;
-                    prev = best;
-                    __syncthreads();
+                for (int o = 16; o; o >>= 1) {
+                    const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, o);
+                    best = best > y ? best : y;
                 }
-                if (warp == 0) list = merge32(list, found, lane);
+                if (lane == 0) s_best[warp] = best;
+                __syncthreads();
+                for (int w = 0; w < NW; ++w) best = best > s_best[w] ? best : s_best[w];
+                if (threadIdx.x == 0) list[j] = best;
+                prev = best;
+                __syncthreads();
             }
-            if (warp == 0) {
-                const unsigned long long kth = __shfl_sync(0xffffffffu, list, k - 1);
-                __syncwarp();
-                if (lane == 0) {
-                    s_count[turn ^ 1] = 0;
-                    s_kth = kth ? order_value(kth) : -CUDART_INF_F;
-                }
-            }
+            if (warp == 0 && lane >= k) list[lane] = 0ull;
         }
-        if (!k) __syncthreads();  // s_max has been read before the next step writes it
     }
     // a NaN target comes behind what is not NaN, a -inf one behind what is larger; of its own kind, behind lower columns
     if (inside && !ordinary) {
-        for (uint32_t i = lo + part * 32 * NW + threadIdx.x; i < hi; i += a.cluster * 32 * NW) {
+        for (int64_t i = lo + (int64_t)(part * 32 * NW + threadIdx.x); i < hi; i += a.cluster * 32 * NW) {
             const float e = load_logit<BF>(a.logits, base + i);
             const bool same = xt == xt ? e == xt : e != e;
             p.ahead += same ? i < t : e > xt || (xt != xt && e == e);
@@ -392,30 +504,43 @@ __global__ void __launch_bounds__(32 * NW, LOGPROBS_WARPS / NW) logprobs_kernel(
             p.ahead += s_part[w].ahead;
         }
     }
-    if (a.cluster > 1) {
-        if (warp == 0) {
-            s_list[lane] = list;
-            if (lane == 0) s_cta = p;
-        }
+    if (NW == kMostWarps && a.cluster > 1) {
+        if (threadIdx.x == 0) s_cta = p;
+        if (warp == 0 && current) s_list[0][lane] = s_list[1][lane];  // peers look at the first
         cluster_sync();
-        if (part == 0 && warp == 0) {
-            for (uint32_t r = 1; r < a.cluster; ++r) {
-                Part o;
-                o.m = __uint_as_float(ld_peer(&s_cta.m, r));
-                o.s = __uint_as_float(ld_peer(&s_cta.s, r));
-                o.c = __uint_as_float(ld_peer(&s_cta.c, r));
-                o.d = __uint_as_float(ld_peer(&s_cta.d, r));
-                o.ahead = ld_peer(&s_cta.ahead, r);
-                p = merge(p, o);
-                if (k) {
-                    const uint32_t* peer = reinterpret_cast<const uint32_t*>(&s_list[lane]);
-                    const unsigned long long l = ld_peer(peer, r), h = ld_peer(peer + 1, r);
-                    list = merge32(list, h << 32 | l, lane);
+        if (part == 0) {
+            if (warp == 0) {
+                for (uint32_t r = 1; r < a.cluster; ++r) {
+                    Part o;
+                    o.m = __uint_as_float(ld_peer(&s_cta.m, r));
+                    o.s = __uint_as_float(ld_peer(&s_cta.s, r));
+                    o.c = __uint_as_float(ld_peer(&s_cta.c, r));
+                    o.d = __uint_as_float(ld_peer(&s_cta.d, r));
+                    o.ahead = ld_peer(&s_cta.ahead, r);
+                    p = merge(p, o);
                 }
+            }
+            if (k && warp < a.cluster) {  // a warp fetches a CTA's list
+                const uint32_t* peer = reinterpret_cast<const uint32_t*>(&s_list[0][lane]);
+                const unsigned long long l = ld_peer(peer, warp), h = ld_peer(peer + 1, warp);
+                s_cand[threadIdx.x] = h << 32 | l;
             }
         }
         cluster_sync();  // the peers' shared memory has been read
         if (part != 0) return;
+        current = 0;
+        if (k) {
+            const unsigned long long mine = warp < a.cluster && lane < k ? s_cand[threadIdx.x] : 0ull;
+            if (warp == 0) s_list[0][lane] = 0ull;
+            __syncthreads();
+            if (mine) {
+                uint32_t place = 0;
+                for (uint32_t r = 0; r < a.cluster; ++r)
+                    for (uint32_t i = 0; i < k; ++i) place += s_cand[32 * r + i] > mine;
+                if (place < 32) s_list[0][place] = mine;
+            }
+            __syncthreads();
+        }
     }
     if (warp != 0) return;
     const bool nothing = !(p.m > -CUDART_INF_F && p.m < CUDART_INF_F) || p.s != p.s;
@@ -423,14 +548,23 @@ __global__ void __launch_bounds__(32 * NW, LOGPROBS_WARPS / NW) logprobs_kernel(
     if (lane == 0) {
         a.logprob[row] = nothing ? CUDART_NAN_F : (float)((double)xt - (double)p.m - lse);
         a.entropy[row] = nothing ? CUDART_NAN_F : (float)(lse + (double)p.d / (1.0 + s));
-        a.rank[row] = inside ? p.ahead : n;
+        a.rank[row] = inside ? p.ahead : (uint32_t)n;
     }
     if (lane < k) {
-        a.top_ids[(uint64_t)row * k + lane] = list ? ~(uint32_t)list : 0xffffffffu;
+        const unsigned long long o = s_list[current][lane];
+        a.top_ids[(uint64_t)row * k + lane] = o ? ~(uint32_t)o : 0xffffffffu;
         float lp = -CUDART_INF_F;
-        if (list) lp = nothing ? CUDART_NAN_F : (float)((double)order_value(list) - (double)p.m - lse);
+        if (o) lp = nothing ? CUDART_NAN_F : (float)((double)order_value(o) - (double)p.m - lse);
         a.top_logprobs[(uint64_t)row * k + lane] = lp;
     }
+}
+
+template <int NW>
+constexpr uint32_t kStepBytes = NW * 32 * kVecs * 16;
+
+template <bool BF, int NW>
+cudaError_t configure() {
+    return cudaFuncSetAttribute(logprobs_kernel<BF, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kStepBytes<NW>);
 }
 
 template <bool BF, int NW>
@@ -438,6 +572,9 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(a.rows * a.cluster);
     cfg.blockDim = dim3(32 * NW);
+    // a second step's room only where a row has one
+    const uint64_t bytes = (uint64_t)a.choices * (BF ? 2 : 4) + 16;
+    cfg.dynamicSmemBytes = kStepBytes<NW> * (bytes > (uint64_t)kStepBytes<NW> * a.cluster ? 2 : 1);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -456,12 +593,16 @@ cudaError_t launch_warps(const Args& a, uint32_t warps, cudaStream_t stream) {
         case 1: return launch<BF, 1>(a, stream);
         case 2: return launch<BF, 2>(a, stream);
         case 4: return launch<BF, 4>(a, stream);
-        case 8: return launch<BF, 8>(a, stream);
-        default: return launch<BF, 16>(a, stream);
+        default: return launch<BF, kMostWarps>(a, stream);
     }
 }
 
 }  // namespace
+
+cudaError_t configure_logprobs_kernels() {  // beyond 48 KB only these
+    cudaError_t e = configure<true, kMostWarps>();
+    return e != cudaSuccess ? e : configure<false, kMostWarps>();
+}
 
 cudaError_t launch_token_logprobs(const LogprobsLaunch& L, cudaStream_t stream) {
     Args a{};
@@ -481,8 +622,8 @@ cudaError_t launch_token_logprobs(const LogprobsLaunch& L, cudaStream_t stream) 
     a.cluster = 1;
     // As many warps as the row has 4 KB, up to 16; with too few rows to give
     // every SM one, 8 warps and a cluster of CTAs for what is longer.
-    const uint64_t parts = ((uint64_t)L.choices * (L.bf16 ? 2 : 4) + 16 + 4095) / 4096;
-    const uint32_t most = L.rows < L.num_sms ? 8u : 16u;
+    const uint64_t parts = ((uint64_t)L.choices * (L.bf16 ? 2 : 4) + 4095) / 4096;
+    const uint32_t most = kMostWarps;
     uint32_t warps = 1;
     while (warps < most && warps < parts) warps *= 2;
     while (a.cluster < 8 && (uint64_t)L.rows * a.cluster * 2 <= 2ull * L.num_sms && (uint64_t)warps * a.cluster < parts)
