@@ -78,7 +78,6 @@ int32_t device_info(DeviceInfo& out) {
                         d.major, minor);
         if ((e = pp::configure_attention_kernels(dev)) != cudaSuccess) return cuda_fail(e, "kernel configuration");
         if ((e = pp::configure_prompt_kernels()) != cudaSuccess) return cuda_fail(e, "kernel configuration");
-        if ((e = pp::configure_logprobs_kernels()) != cudaSuccess) return cuda_fail(e, "kernel configuration");
         if (!g_encode) {
             void* fn = nullptr;
             cudaDriverEntryPointQueryResult q{};

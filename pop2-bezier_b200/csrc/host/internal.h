@@ -239,7 +239,6 @@ struct LogprobsLaunch {
 };
 
 cudaError_t launch_prompt_append(const PromptAppendLaunch& P, cudaStream_t stream);
-cudaError_t configure_logprobs_kernels();
 cudaError_t launch_token_logprobs(const LogprobsLaunch& L, cudaStream_t stream);
 
 // QKV RoPE (+ int8 append): see decoder.cu.

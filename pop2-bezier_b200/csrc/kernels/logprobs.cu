@@ -11,10 +11,11 @@
 // (d + g (s + count)) exp(-g).
 //
 // A thread copies 8 vectors of 16 bytes into shared memory (cp.async) and looks at
-// them several times (maximum, sums, rank, alternatives) in short loops, while its
-// next 8 are on their way: nothing waits for another thread's copies, and the
-// loops stay in the instruction cache, which the same code unrolled over
-// registers did not (4096 rows of 32768: 154 us).  NW warps take 4 KB each of a
+// them several times (maximum, sums, rank, alternatives) in short loops: nothing
+// waits for another thread's copies, and the loops stay in the instruction cache,
+// which the same code unrolled over registers did not (4096 rows of 32768: 154 us
+// against 95).  One buffer a CTA leaves room for five CTAs an SM, which hide the
+// copies better than a second buffer with three (117 us).  NW warps take 4 KB each of a
 // row; a longer row is taken in steps, with one barrier each, or by a cluster of
 // up to 8 CTAs that merge through their shared memory, when there are few rows.
 //
@@ -55,7 +56,7 @@ struct Args {
     uint32_t* status;
 };
 
-// What a CTA (or a thread, with its own s, c, d and ahead) knows of a row.
+// What a thread or a CTA knows of a row; the threads of a CTA have one m.
 struct Part {
     float m, s, c, d;
     uint32_t ahead;
@@ -75,17 +76,6 @@ __device__ __forceinline__ void raise(Part& p, float m) {
     }
     p.c = 0.f;
     p.m = m;
-}
-
-__device__ __forceinline__ Part merge(Part a, Part b) {
-    const float m = fmaxf(a.m, b.m);
-    raise(a, m);
-    raise(b, m);
-    a.s += b.s;
-    a.c += b.c;
-    a.d += b.d;
-    a.ahead += b.ahead;
-    return a;
 }
 
 // Order of the alternatives as one number: larger logit, then lower column.
@@ -189,10 +179,7 @@ __device__ __forceinline__ void copy16(uint4* to, const void* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(to)), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_sent() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LATER>
-__device__ __forceinline__ void copies_landed() {  // all but the last LATER groups
-    asm volatile("cp.async.wait_group %0;" ::"n"(LATER) : "memory");
-}
+__device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
 // The list of the best 32 from the candidates and the list before it, by all of the block.
 __device__ __noinline__ void sort_candidates(const unsigned long long* cand, uint32_t count,
@@ -216,7 +203,7 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
     constexpr int EPV = BF ? 8 : 4;                    // elements of a vector
     constexpr uint32_t T = 32 * NW, STEP = T * kVecs;  // vectors a CTA takes at a time
     constexpr int kLow = (int)0x807fffff;              // rising(-inf)
-    extern __shared__ uint4 s_row[];                   // one or two steps, vector v of thread t at v T + t
+    extern __shared__ uint4 s_row[];                   // a step, vector v of thread t at v T + t
     __shared__ int s_top[2][NW], s_reached[2][NW];
     __shared__ unsigned long long s_cand[NW * kCandidates], s_list[2][32], s_best[NW];
     __shared__ uint32_t s_count;
@@ -244,34 +231,38 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
     const int first = lo - (int)((reinterpret_cast<uint64_t>(row_ptr) + (uint64_t)lo * (BF ? 2 : 4)) % 16 / (BF ? 2 : 4));
     const uint32_t vectors = n ? ((uint32_t)(hi - first) + EPV - 1) / EPV : 0u;
 
-    auto fetch = [&](uint32_t v0, uint4* to) {
-#pragma unroll 4
-        for (int v = 0; v < kVecs; ++v) {
+    auto fetch = [&](uint32_t v0) {
+        uint4* to = s_row + threadIdx.x;
+        const int col0 = first + (int)(v0 + threadIdx.x) * EPV;
+        const char* from = row_ptr + (int64_t)col0 * (BF ? 2 : 4);
+        if (first + (int)v0 * EPV >= lo && v0 + STEP <= vectors && first + (int)(v0 + STEP) * EPV <= hi) {
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v) copy16(to + v * T, from + v * T * 16);
+            copies_sent();
+            return;
+        }
+#pragma unroll 1
+        for (int v = 0; v < kVecs; ++v, to += T, from += T * 16) {
             const uint32_t at = v0 + v * T + threadIdx.x;
-            const int col = first + (int)at * EPV;
+            const int col = col0 + v * T * EPV;
             if (at < vectors && col >= lo && col + EPV <= hi) {
-                copy16(to + v * T + threadIdx.x, row_ptr + (int64_t)col * (BF ? 2 : 4));
-            } else {  // an end of the window, or nothing
-                const uint32_t none = BF ? 0xff80ff80u : 0xff800000u;  // -inf
-                uint4 y = make_uint4(none, none, none, none);
-                to[v * T + threadIdx.x] = y;
-                if (at < vectors) {
-                    for (int i = 0; i < EPV; ++i)
-                        if (col + i >= lo && col + i < hi) {
-                            const uint32_t bits = __float_as_uint(load_logit<BF>(a.logits, base + col + i));
-                            if constexpr (BF)
-                                reinterpret_cast<uint16_t*>(to + v * T + threadIdx.x)[i] = (uint16_t)(bits >> 16);
-                            else reinterpret_cast<uint32_t*>(to + v * T + threadIdx.x)[i] = bits;
-                        }
-                }
+                copy16(to, from);
+                continue;
             }
+            const uint32_t none = BF ? 0xff80ff80u : 0xff800000u;  // -inf: an end of the window, or nothing
+            *to = make_uint4(none, none, none, none);
+            if (at >= vectors) continue;
+            for (int i = 0; i < EPV; ++i)
+                if (col + i >= lo && col + i < hi) {
+                    const uint32_t bits = __float_as_uint(load_logit<BF>(a.logits, base + col + i));
+                    if constexpr (BF) reinterpret_cast<uint16_t*>(to)[i] = (uint16_t)(bits >> 16);
+                    else reinterpret_cast<uint32_t*>(to)[i] = bits;
+                }
         }
         copies_sent();
     };
     const uint32_t stride = a.cluster * STEP;
-    uint4* now = s_row;
-    uint4* later = s_row + STEP;
-    if (part * STEP < vectors) fetch(part * STEP, now);
+    if (part * STEP < vectors) fetch(part * STEP);
 
     const int t = a.targets[row];
     const bool inside = t >= lo && t < hi;
@@ -280,6 +271,7 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
     const bool ordinary = inside && xt > -CUDART_INF_F;
 
     Part p{-CUDART_INF_F, 0.f, 0.f, 0.f, 0u};
+    const uint4* x = s_row + threadIdx.x;
     uint32_t turn = 0;     // steps take turns at what the warps tell each other
     uint32_t current = 0;  // which of the two lists is the last one
     uint32_t found = 0;    // candidates of the warp
@@ -287,16 +279,20 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
     bool over = false;  // candidates did not fit: the list is found in the row again
     __syncthreads();
     for (uint32_t v0 = part * STEP; v0 < vectors; v0 += stride, turn ^= 1) {
-        if (v0 + stride < vectors) {
-            fetch(v0 + stride, later);
-            copies_landed<1>();
-        } else {
-            copies_landed<0>();
-        }
-        const uint4* x = now + threadIdx.x;
+        copies_landed();
         float top = -CUDART_INF_F;
-#pragma unroll 4
-        for (int v = 0; v < kVecs; ++v) top = fmaxf(top, vector_max<BF>(x[v * T]));
+        if constexpr (BF) {
+            uint32_t most = 0xff80ff80u;
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v) {
+                const uint4 y = x[v * T];
+                most = max_bf16x2(max_bf16x2(most, max_bf16x2(y.x, y.y)), max_bf16x2(y.z, y.w));
+            }
+            top = fmaxf(bf16_lo_to_f32(most), bf16_hi_to_f32(most));
+        } else {
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v) top = fmaxf(top, vector_max<false>(x[v * T]));
+        }
         const int key = rising(top);
         const int warp_key = __reduce_max_sync(0xffffffffu, key);
         const float warp_top = rising_value(warp_key);
@@ -341,53 +337,76 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
         const float ref = m > -CUDART_INF_F ? m : 0.f;  // nothing but -inf so far (or NaN, which has to show in s)
         const float r = ref * kLog2e, slip = fmaf(ref, kLog2e, -r);
         const uint64_t neg = f2_pack(-r, -r), l2e = f2_pack(kLog2e, kLog2e);
-        uint64_t s0 = 0ull, s1 = 0ull, d0 = 0ull, d1 = 0ull;
-        uint32_t ahead2 = 0;  // two bf16 counts, at most 32 each
-        const bool look = ordinary && warp_top >= xt;
         // No x is taken below `low`, at least 119 under the maximum also as bf16: exp2 of its y is 0, and so is their
-        // product, which that of -inf would not be.  Beyond 2^20 the slip is no small number: one by one then.
+        // product, which that of -inf would not be.  Beyond 2^20 the slip is no small number.
         const float low = ref - 120.f - 0.01f * fabsf(ref);
         const bool plain = fabsf(ref) < 1048576.f;
-        const uint32_t low2 = pack_bf16x2(low, low), xt2 = pack_bf16x2(xt, xt);
-#pragma unroll 2
-        for (int v = 0; v < kVecs; ++v) {
-            const uint4 y4 = x[v * T];
+        const uint32_t low2 = pack_bf16x2(low, low);
+        uint64_t s0 = 0ull, s1 = 0ull, d0 = 0ull, d1 = 0ull;
+        auto add = [&](const uint4& y4) {
             const uint32_t w[4] = {y4.x, y4.y, y4.z, y4.w};
-            const float vm = vector_max<BF>(y4);
-            const int col = first + (int)(v0 + v * T + threadIdx.x) * EPV;
-            if (vm == m || !plain) {  // holds the maximum: it is counted, not summed
+#pragma unroll
+            for (int i = 0; i < EPV; i += 2) {
+                float x0, x1, y0, y1;
+                if constexpr (BF) {
+                    uint32_t u;
+                    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(u) : "r"(w[i / 2]), "r"(low2));
+                    x0 = bf16_lo_to_f32(u);
+                    x1 = bf16_hi_to_f32(u);
+                } else {
+                    asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(__uint_as_float(w[i])), "f"(low));
+                    asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(__uint_as_float(w[i + 1])), "f"(low));
+                }
+                uint64_t y2;
+                asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y2) : "l"(f2_pack(x0, x1)), "l"(l2e), "l"(neg));
+                f2_unpack(y2, y0, y1);
+                const uint64_t e2 = f2_pack(fast_exp2(y0), fast_exp2(y1));
+                uint64_t& s = i & 2 ? s1 : s0;
+                uint64_t& d = i & 2 ? d1 : d0;
+                s = f2_add(s, e2);
+                asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(e2), "l"(y2));
+            }
+        };
+        if (warp_top < m && plain) {
+#pragma unroll 2
+            for (int v = 0; v < kVecs; ++v) add(x[v * T]);
+        } else {  // the warp holds the maximum, which is counted, not summed (or -inf and NaN only, or huge numbers)
 #pragma unroll 1
+            for (int v = 0; v < kVecs; ++v) {
+                const uint4 y4 = x[v * T];
+                if (vector_max<BF>(y4) < m && plain) {
+                    add(y4);
+                    continue;
+                }
+                float es[2] = {0.f, 0.f}, ed[2] = {0.f, 0.f};
+#pragma unroll
                 for (int i = 0; i < EPV; ++i) {
-                    const float e = picked<BF>(x + v * T, i);
+                    const float e = element<BF>(y4, i);
                     const float y = fmaxf((e - ref) * kLog2e, -160.f), f = e == m ? 0.f : fast_exp2(e == e ? y : e);
                     p.c += e == m ? 1.f : 0.f;
-                    p.s += f;
-                    p.d -= f * y * 0.6931471805599453f;
+                    es[i & 1] += f;
+                    ed[i & 1] += f * y;
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < EPV; i += 2) {
-                    float x0, x1, y0, y1;
-                    if constexpr (BF) {
-                        uint32_t u;
-                        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(u) : "r"(w[i / 2]), "r"(low2));
-                        x0 = bf16_lo_to_f32(u);
-                        x1 = bf16_hi_to_f32(u);
-                    } else {
-                        asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(__uint_as_float(w[i])), "f"(low));
-                        asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(__uint_as_float(w[i + 1])), "f"(low));
-                    }
-                    uint64_t y2;
-                    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y2) : "l"(f2_pack(x0, x1)), "l"(l2e), "l"(neg));
-                    f2_unpack(y2, y0, y1);
-                    const uint64_t e2 = f2_pack(fast_exp2(y0), fast_exp2(y1));
-                    uint64_t& s = i & 2 ? s1 : s0;
-                    uint64_t& d = i & 2 ? d1 : d0;
-                    s = f2_add(s, e2);
-                    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(e2), "l"(y2));
-                }
+                p.s += es[0] + es[1];
+                p.d -= (ed[0] + ed[1]) * 0.6931471805599453f;
             }
-            if (look && vm >= xt) {
+        }
+        if (plain) {
+            float e0, e1, e2, e3;
+            f2_unpack(f2_add(s0, s1), e0, e1);
+            f2_unpack(f2_add(d0, d1), e2, e3);
+            const float sum = e0 + e1, back = fast_exp2(-slip);
+            p.s += sum * back;
+            p.d -= (e2 + e3 - slip * sum) * back * 0.6931471805599453f;
+        }
+        if (ordinary && warp_top >= xt) {
+            const uint32_t xt2 = pack_bf16x2(xt, xt);
+            uint32_t ahead2 = 0;  // two bf16 counts, at most 32 each
+#pragma unroll 2
+            for (int v = 0; v < kVecs; ++v) {
+                const uint4 y4 = x[v * T];
+                const uint32_t w[4] = {y4.x, y4.y, y4.z, y4.w};
+                const int col = first + (int)(v0 + v * T + threadIdx.x) * EPV;
                 if (col <= t && t < col + EPV) {
 #pragma unroll 1
                     for (int i = 0; i < EPV; ++i) {
@@ -395,7 +414,6 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
                         p.ahead += e > xt || (e == xt && col + i < t);
                     }
                 } else if constexpr (BF) {
-                    // x >= xt is x > the bf16 below xt, but not at the ends of the type: two loops
                     if (col < t) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) ahead2 = add_bf16x2(ahead2, above_bf16x2<true>(w[i], xt2));
@@ -411,7 +429,15 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
                     }
                 }
             }
-            if (k && __any_sync(0xffffffffu, vm >= bound && vm > -CUDART_INF_F)) {
+            if constexpr (BF) p.ahead += (uint32_t)(bf16_lo_to_f32(ahead2) + bf16_hi_to_f32(ahead2));
+        }
+        if (k && __any_sync(0xffffffffu, top >= bound && top > -CUDART_INF_F)) {
+#pragma unroll 1
+            for (int v = 0; v < kVecs; ++v) {
+                const uint4 y4 = x[v * T];
+                const float vm = vector_max<BF>(y4);
+                if (!__any_sync(0xffffffffu, vm >= bound && vm > -CUDART_INF_F)) continue;
+                const int col = first + (int)(v0 + v * T + threadIdx.x) * EPV;
                 uint32_t have = 0;  // candidates of the lane's vector, as bits
 #pragma unroll
                 for (int i = 0; i < EPV; ++i) {
@@ -430,18 +456,7 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
                 }
             }
         }
-        if constexpr (BF) p.ahead += (uint32_t)(bf16_lo_to_f32(ahead2) + bf16_hi_to_f32(ahead2));
-        if (plain) {
-            float e0, e1, e2, e3;
-            f2_unpack(f2_add(s0, s1), e0, e1);
-            f2_unpack(f2_add(d0, d1), e2, e3);
-            const float sum = e0 + e1, back = fast_exp2(-slip);
-            p.s += sum * back;
-            p.d -= (e2 + e3 - slip * sum) * back * 0.6931471805599453f;
-        }
-        uint4* done = now;
-        now = later;
-        later = done;
+        if (v0 + stride < vectors) fetch(v0 + stride);
     }
     if (k) {
         over = __syncthreads_or(found > kCandidates) || over;
@@ -496,12 +511,14 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
     }
     if (lane == 0) s_part[warp] = p;
     __syncthreads();
-    if (warp == 0) {
-        for (int w = 1; w < NW; ++w) {
-            p.s += s_part[w].s;
-            p.c += s_part[w].c;
-            p.d += s_part[w].d;
-            p.ahead += s_part[w].ahead;
+    if (warp == 0 && NW > 1) {
+        p = lane < NW ? s_part[lane] : Part{p.m, 0.f, 0.f, 0.f, 0u};
+#pragma unroll
+        for (int o = NW / 2; o; o >>= 1) {
+            p.s += __shfl_xor_sync(0xffffffffu, p.s, o);
+            p.c += __shfl_xor_sync(0xffffffffu, p.c, o);
+            p.d += __shfl_xor_sync(0xffffffffu, p.d, o);
+            p.ahead += __shfl_xor_sync(0xffffffffu, p.ahead, o);
         }
     }
     if (NW == kMostWarps && a.cluster > 1) {
@@ -509,62 +526,64 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
         if (warp == 0 && current) s_list[0][lane] = s_list[1][lane];  // peers look at the first
         cluster_sync();
         if (part == 0) {
-            if (warp == 0) {
-                for (uint32_t r = 1; r < a.cluster; ++r) {
-                    Part o;
-                    o.m = __uint_as_float(ld_peer(&s_cta.m, r));
-                    o.s = __uint_as_float(ld_peer(&s_cta.s, r));
-                    o.c = __uint_as_float(ld_peer(&s_cta.c, r));
-                    o.d = __uint_as_float(ld_peer(&s_cta.d, r));
-                    o.ahead = ld_peer(&s_cta.ahead, r);
-                    p = merge(p, o);
+            if (warp == 0) {  // lane r fetches CTA r's part
+                if (lane < a.cluster && lane) {
+                    const float ms = __uint_as_float(ld_peer(&s_cta.m, lane)), ss = __uint_as_float(ld_peer(&s_cta.s, lane));
+                    const float cs = __uint_as_float(ld_peer(&s_cta.c, lane)), ds = __uint_as_float(ld_peer(&s_cta.d, lane));
+                    p = Part{ms, ss, cs, ds, ld_peer(&s_cta.ahead, lane)};
+                } else if (lane) {
+                    p = Part{-CUDART_INF_F, 0.f, 0.f, 0.f, 0u};
+                }
+                float m = p.m;
+#pragma unroll
+                for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                raise(p, m);
+#pragma unroll
+                for (int o = 4; o; o >>= 1) {
+                    p.s += __shfl_xor_sync(0xffffffffu, p.s, o);
+                    p.c += __shfl_xor_sync(0xffffffffu, p.c, o);
+                    p.d += __shfl_xor_sync(0xffffffffu, p.d, o);
+                    p.ahead += __shfl_xor_sync(0xffffffffu, p.ahead, o);
                 }
             }
-            if (k && warp < a.cluster) {  // a warp fetches a CTA's list
+            if (k && warp < a.cluster && lane < k) {  // a warp fetches a CTA's list
                 const uint32_t* peer = reinterpret_cast<const uint32_t*>(&s_list[0][lane]);
                 const unsigned long long l = ld_peer(peer, warp), h = ld_peer(peer + 1, warp);
-                s_cand[threadIdx.x] = h << 32 | l;
+                s_cand[warp * k + lane] = h << 32 | l;
             }
         }
         cluster_sync();  // the peers' shared memory has been read
         if (part != 0) return;
-        current = 0;
         if (k) {
-            const unsigned long long mine = warp < a.cluster && lane < k ? s_cand[threadIdx.x] : 0ull;
-            if (warp == 0) s_list[0][lane] = 0ull;
-            __syncthreads();
-            if (mine) {
-                uint32_t place = 0;
-                for (uint32_t r = 0; r < a.cluster; ++r)
-                    for (uint32_t i = 0; i < k; ++i) place += s_cand[32 * r + i] > mine;
-                if (place < 32) s_list[0][place] = mine;
+            if (warp == 0) {
+                s_list[0][lane] = 0ull;
+                s_list[1][lane] = 0ull;
             }
+            __syncthreads();
+            // missing entries are 0 and land behind the others, where the list is 0
+            sort_candidates(s_cand, a.cluster * k, s_list[0], s_list[1], k);
+            current = 1;
             __syncthreads();
         }
     }
     if (warp != 0) return;
+    p.s = __shfl_sync(0xffffffffu, p.s, 0);  // lane 0 has the row's; all of them write alternatives
+    p.c = __shfl_sync(0xffffffffu, p.c, 0);
+    p.m = __shfl_sync(0xffffffffu, p.m, 0);
     const bool nothing = !(p.m > -CUDART_INF_F && p.m < CUDART_INF_F) || p.s != p.s;
-    const double s = (double)p.s + (double)(p.c - 1.f), lse = log1p(s);  // of the sum, less m
+    const float s = p.s + (p.c - 1.f), lse = log1pf(s);  // of the sum, less m
     if (lane == 0) {
-        a.logprob[row] = nothing ? CUDART_NAN_F : (float)((double)xt - (double)p.m - lse);
-        a.entropy[row] = nothing ? CUDART_NAN_F : (float)(lse + (double)p.d / (1.0 + s));
+        a.logprob[row] = nothing ? CUDART_NAN_F : (xt - p.m) - lse;
+        a.entropy[row] = nothing ? CUDART_NAN_F : lse + p.d / (1.f + s);
         a.rank[row] = inside ? p.ahead : (uint32_t)n;
     }
     if (lane < k) {
         const unsigned long long o = s_list[current][lane];
         a.top_ids[(uint64_t)row * k + lane] = o ? ~(uint32_t)o : 0xffffffffu;
         float lp = -CUDART_INF_F;
-        if (o) lp = nothing ? CUDART_NAN_F : (float)((double)order_value(o) - (double)p.m - lse);
+        if (o) lp = nothing ? CUDART_NAN_F : (order_value(o) - p.m) - lse;
         a.top_logprobs[(uint64_t)row * k + lane] = lp;
     }
-}
-
-template <int NW>
-constexpr uint32_t kStepBytes = NW * 32 * kVecs * 16;
-
-template <bool BF, int NW>
-cudaError_t configure() {
-    return cudaFuncSetAttribute(logprobs_kernel<BF, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kStepBytes<NW>);
 }
 
 template <bool BF, int NW>
@@ -572,9 +591,7 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(a.rows * a.cluster);
     cfg.blockDim = dim3(32 * NW);
-    // a second step's room only where a row has one
-    const uint64_t bytes = (uint64_t)a.choices * (BF ? 2 : 4) + 16;
-    cfg.dynamicSmemBytes = kStepBytes<NW> * (bytes > (uint64_t)kStepBytes<NW> * a.cluster ? 2 : 1);
+    cfg.dynamicSmemBytes = NW * 32 * kVecs * 16;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -598,11 +615,6 @@ cudaError_t launch_warps(const Args& a, uint32_t warps, cudaStream_t stream) {
 }
 
 }  // namespace
-
-cudaError_t configure_logprobs_kernels() {  // beyond 48 KB only these
-    cudaError_t e = configure<true, kMostWarps>();
-    return e != cudaSuccess ? e : configure<false, kMostWarps>();
-}
 
 cudaError_t launch_token_logprobs(const LogprobsLaunch& L, cudaStream_t stream) {
     Args a{};

@@ -131,22 +131,30 @@ def _starts(t: torch.Tensor, n: int | None, device: torch.device) -> int:
     return t.numel() - 1
 
 
+_PROMPT_DTYPES = {torch.float32: N.DTYPE_F32, torch.bfloat16: N.DTYPE_BF16}
+
+
 def prompt_struct(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sequences: int, *, causal: bool = True,
                   softmax_scale: float = 0.0, plan_ready: bool = False, max_ctas: int = 0) -> N.PpPrompt:
     """The C ABI's geometry of packed prompts, after its checks."""
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
+    kshape, dt = k.shape, q.dtype
+    if q.dim() != 3 or len(kshape) != 3 or v.shape != kshape:
         raise N.PreconditionError(_MSG_PROMPT)
     tokens, heads, d = q.shape
-    kv_tokens, kv_heads, kd = k.shape
-    dt = q.dtype
-    if not q.is_cuda or k.device != q.device or v.device != q.device or kd != d or d not in (64, 128) \
-            or dt not in (torch.float32, torch.bfloat16) or k.dtype != dt or v.dtype != dt or heads == 0 or kv_heads == 0 \
-            or heads % kv_heads or heads > 64 * kv_heads or q.stride(2) != 1 or k.stride(2) != 1 or v.stride(2) != 1:
+    kv_tokens, kv_heads, kd = kshape
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    code = _PROMPT_DTYPES.get(dt)
+    dev = q.get_device() if q.is_cuda else -1
+    if dev < 0 or k.get_device() != dev or v.get_device() != dev or kd != d or (d != 64 and d != 128) or code is None \
+            or k.dtype != dt or v.dtype != dt or heads == 0 or kv_heads == 0 or heads % kv_heads or heads > 64 * kv_heads \
+            or qs[2] != 1 or ks[2] != 1 or vs[2] != 1:
         raise N.PreconditionError(_MSG_PROMPT)
-    return N.PpPrompt(C.sizeof(N.PpPrompt), sequences, heads, kv_heads, d,
-                      N.DTYPE_F32 if dt == torch.float32 else N.DTYPE_BF16, tokens, kv_tokens, int(bool(causal)),
-                      softmax_scale, N.ATTN_PLAN_READY if plan_ready else 0, max_ctas, q.stride(0), q.stride(1),
-                      k.stride(0), k.stride(1), v.stride(0), v.stride(1), q.data_ptr(), k.data_ptr(), v.data_ptr())
+    return N.PpPrompt(_PROMPT_BYTES, sequences, heads, kv_heads, d, code, tokens, kv_tokens, 1 if causal else 0,
+                      softmax_scale, N.ATTN_PLAN_READY if plan_ready else 0, max_ctas, qs[0], qs[1], ks[0], ks[1], vs[0],
+                      vs[1], q.data_ptr(), k.data_ptr(), v.data_ptr())
+
+
+_PROMPT_BYTES = C.sizeof(N.PpPrompt)
 
 
 def prompt_workspace(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sequences: int, *, max_ctas: int = 0
@@ -155,7 +163,7 @@ def prompt_workspace(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sequence
     shapes and that many sequences.  Calls that may run at the same time need
     one each."""
     g = prompt_struct(q, k, v, sequences, max_ctas=max_ctas)
-    with torch.cuda.device(q.device):
+    with ops._here(q):
         return torch.empty(int(N.lib.pp_b200_prompt_workspace_size(C.byref(g))), dtype=torch.uint8, device=q.device)
 
 
@@ -170,7 +178,7 @@ def plan_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts: tor
         _starts(kv_starts, n, q.device)
     g = prompt_struct(q, k, v, n, causal=causal, max_ctas=max_ctas)
     _prompt_buffers(q, workspace, status)
-    with torch.cuda.device(q.device):
+    with ops._here(q):
         N.check(N.lib.pp_b200_plan_prompt(C.byref(g), q_starts.data_ptr(), ops._ptr(kv_starts), workspace.data_ptr(),
                                           workspace.numel(), ops._ptr(status), ops._stream(q)))
 
@@ -209,10 +217,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts
     if plan_ready and workspace is None:
         raise N.PreconditionError("plan_ready needs the workspace that plan_prompt wrote")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
         raise N.PreconditionError("prompt attention writes a dense [tokens,heads,head_dim] of q's type and device")
-    with torch.cuda.device(q.device):
+    with ops._here(q):
         if workspace is None:
             workspace = torch.empty(N.lib.pp_b200_prompt_workspace_size(C.byref(g)), dtype=torch.uint8, device=q.device)
         N.check(N.lib.pp_b200_prompt_attention(C.byref(g), q_starts.data_ptr(), ops._ptr(kv_starts), out.data_ptr(),

@@ -144,7 +144,7 @@ class Int8KvArena:
                 raise N.PreconditionError("prompt starts and offsets must be contiguous U32")
         code = ops._dtype_code(k, "K/V input")
         a = self.struct()
-        with torch.cuda.device(k.device):
+        with ops._here(k):
             N.check(N.lib.pp_b200_prompt_append(C.byref(a), k.data_ptr(), v.data_ptr(), code, k.shape[0], k.stride(0),
                                                 k.stride(1), v.stride(0), v.stride(1), starts.data_ptr(),
                                                 offsets.data_ptr(), ops._ptr(status), ops._stream(k)))

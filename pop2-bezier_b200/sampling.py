@@ -72,7 +72,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0,
     if logits.dim() != 2 or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise N.PreconditionError("token logprobs need logits [rows, choices] with contiguous rows and a nonempty head")
     rows, choices = logits.shape
-    if targets.numel() != rows or targets.dtype != torch.int32 or not targets.is_contiguous():
+    if targets.dim() != 1 or targets.numel() != rows or targets.dtype != torch.int32 or not targets.is_contiguous():
         raise N.PreconditionError("token logprobs need one contiguous I32 target a row")
     if bounds is not None and (bounds.numel() != 2 * rows or bounds.dtype not in (torch.int32, torch.uint32)
                                or not bounds.is_contiguous()):
@@ -82,11 +82,11 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0,
     code = ops._dtype_code(logits, "logits")
     stride = logits.stride(0) if rows > 1 else choices
     dev = logits.device
-    logprob, entropy = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind(0)
-    rank = torch.empty(rows, dtype=torch.int32, device=dev)
+    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
+    entropy, rank = torch.empty_like(logprob), torch.empty_like(targets)
     ids = torch.empty((rows, top), dtype=torch.int32, device=dev) if top else None
     best = torch.empty((rows, top), dtype=torch.float32, device=dev) if top else None
-    with torch.cuda.device(dev):
+    with ops._here(logits):
         N.check(N.lib.pp_b200_token_logprobs(
             logits.data_ptr(), code, rows, choices, stride, targets.data_ptr(), ops._ptr(bounds), top,
             logprob.data_ptr(), entropy.data_ptr(), rank.data_ptr(), ops._ptr(ids), ops._ptr(best),
