@@ -68,6 +68,12 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
     return r;
 }
 
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 // Exact conversion of the four signed bytes of `w` to f32 pairs (b0, b1) and
 // (b2, b3), as i8x4_to_f32 but with packed subtraction.
 __device__ __forceinline__ void i8x4_to_f32x2(uint32_t w, uint64_t& p01, uint64_t& p23) {

@@ -211,12 +211,6 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
 // q k', pairs of output channels for p v.
 constexpr int kRowsThreads = 256, kBN = 64;
 
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
 template <bool BF>
 __device__ __forceinline__ float4 load4(const void* p, uint64_t i, bool vec) {
     if constexpr (BF) {

@@ -4,6 +4,20 @@
 //   s = max(max|x| / 127, 1e-12)            IEEE f32 division
 //   q = clamp(round_half_even(x / s), -127, 127)
 // This file is compiled with -fmad=false -prec-div=true, as quant.cu.
+//
+// A streaming kernel: 2 bytes in and 1 out an element (bf16).  What bounds it is
+// the issue of the division's instructions, so x / s is Markstein's division with
+// y = RN(1/s) computed once a row, on packed pairs:
+//   q0 = x y,  q1 = q0 + (x - q0 s) y,  q2 = q1 + (x - q1 s) y     (FMAs)
+// q0 is within 1.5 units of the last place of x/s, q1 within (1/2 + 2^-22), and
+// from an estimate nearer than one unit the last step gives RN(x/s) (P. Markstein,
+// IBM J. Res. Dev. 34, 1990).  Nothing over- or underflows where it matters: s is
+// at least 1e-12, and below |x/s| = 1/4 the code is 0 whatever the last bits say.
+// RN(m/127) is taken the same way with RN(1/127), by one step, which is right for
+// all 2^23 mantissas (the tests go through them).  Rounding is the addition of
+// 1.5 * 2^23, whose low byte is the code; with |x| <= max|x| no clamp is needed.
+// A row that is not finite is divided one by one.  (Dividing only near half
+// integers does not pay: quotients of bf16 numbers fall on them too often.)
 #include "common.cuh"
 #include "../host/internal.h"
 
@@ -12,6 +26,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxChunk = 64;  // tokens of a CTA
+constexpr int kE = 16;         // elements of a lane
+constexpr int kRows = 1;       // rows that a lane has in flight; two cost more registers than they hide latency
 
 struct AppendArgs {
     const void* src[2];  // K, V
@@ -25,42 +41,128 @@ struct AppendArgs {
     uint32_t* status;
 };
 
-// A lane holds 8 consecutive elements of a row, D / 8 lanes a row.
+// A lane's 16 elements as they lie in memory.
 template <bool BF>
-__device__ __forceinline__ void load_row8(const void* p, uint64_t i, bool vec, float (&v)[8]) {
-    if constexpr (BF) {
+struct Raw {
+    uint4 w[BF ? 2 : 4];
+};
+
+template <bool BF>
+__device__ __forceinline__ Raw<BF> load_raw(const void* p, uint64_t i, bool vec) {
+    Raw<BF> r;
+    if (vec) {
+        const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) + i * (BF ? 2 : 4));
+#pragma unroll
+        for (int h = 0; h < (BF ? 2 : 4); ++h) r.w[h] = __ldg(s + h);
+    } else if constexpr (BF) {
         const uint16_t* s = reinterpret_cast<const uint16_t*>(p) + i;
-        if (vec) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(s));
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                v[2 * k] = bf16_lo_to_f32(w[k]);
-                v[2 * k + 1] = bf16_hi_to_f32(w[k]);
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = bf16_lo_to_f32(s[k]);
-        }
+        for (int h = 0; h < 2; ++h)
+            r.w[h] = make_uint4(s[8 * h] | (uint32_t)s[8 * h + 1] << 16, s[8 * h + 2] | (uint32_t)s[8 * h + 3] << 16,
+                                s[8 * h + 4] | (uint32_t)s[8 * h + 5] << 16, s[8 * h + 6] | (uint32_t)s[8 * h + 7] << 16);
     } else {
-        const float* s = reinterpret_cast<const float*>(p) + i;
-        if (vec) {
-            const float4 x = __ldg(reinterpret_cast<const float4*>(s)), y = __ldg(reinterpret_cast<const float4*>(s) + 1);
-            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-            v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
-        } else {
+        const uint32_t* s = reinterpret_cast<const uint32_t*>(p) + i;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = s[k];
+        for (int h = 0; h < 4; ++h) r.w[h] = make_uint4(s[4 * h], s[4 * h + 1], s[4 * h + 2], s[4 * h + 3]);
+    }
+    return r;
+}
+
+template <bool BF>
+__device__ __forceinline__ void unpack(const Raw<BF>& r, float (&v)[kE]) {
+#pragma unroll
+    for (int h = 0; h < (BF ? 2 : 4); ++h) {
+        const uint32_t w[4] = {r.w[h].x, r.w[h].y, r.w[h].z, r.w[h].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (BF) {
+                v[8 * h + 2 * k] = bf16_lo_to_f32(w[k]);
+                v[8 * h + 2 * k + 1] = bf16_hi_to_f32(w[k]);
+            } else {
+                v[4 * h + k] = __uint_as_float(w[k]);
+            }
         }
     }
 }
 
-// CTA x takes `chunk` tokens of all heads, K and V.
+// max|x| of a lane's elements; NaN if one is.
+template <bool BF>
+__device__ __forceinline__ float largest(const Raw<BF>& r) {
+    if constexpr (BF) {
+        uint32_t m = 0u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t w[4] = {r.w[h].x, r.w[h].y, r.w[h].z, r.w[h].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[k] & 0x7fff7fffu));
+        }
+        float lo = bf16_lo_to_f32(m);
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(bf16_hi_to_f32(m)));
+        return lo;
+    } else {
+        float m = 0.f;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const uint32_t w[4] = {r.w[h].x, r.w[h].y, r.w[h].z, r.w[h].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(__uint_as_float(w[k]))));
+        }
+        return m;
+    }
+}
+
+__device__ __forceinline__ float over_127(float m) {  // RN(m / 127)
+    const float y = 0x1.020408p-7f, q = m * y;         // y = RN(1 / 127)
+    return __fmaf_rn(__fmaf_rn(-127.f, q, m), y, q);
+}
+
+struct Divided {
+    uint4 codes;
+    float s;
+    bool finite;
+};
+
+// A lane's part of a row that is not finite, as quant_row.cuh: the scale passes over NaN.
+template <int D, bool BF>
+__device__ __noinline__ Divided divided(const void* src, uint64_t from, bool vec) {
+    constexpr int L = D / kE;
+    float v[kE], m = 0.f;
+    bool finite = true;
+    unpack<BF>(load_raw<BF>(src, from, vec), v);
+#pragma unroll
+    for (int k = 0; k < kE; ++k) {
+        finite = finite && isfinite(v[k]);
+        m = fmaxf(m, fabsf(v[k]));
+    }
+    const uint32_t row_lanes = ((1u << L) - 1u) << (threadIdx.x % 32 / L * L);
+#pragma unroll
+    for (int o = L / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(row_lanes, m, o));
+    const float s = fmaxf(__fdiv_rn(m, 127.f), 1e-12f);
+    uint32_t w[kE / 4];
+#pragma unroll
+    for (int k = 0; k < kE; k += 4) {
+        w[k / 4] = 0u;
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+            w[k / 4] |= (uint32_t)(max(-127, min(127, __float2int_rn(__fdiv_rn(v[k + h], s)))) & 0xff) << (8 * h);
+    }
+    return Divided{make_uint4(w[0], w[1], w[2], w[3]), s, finite};
+}
+
+// CTA (x, y) takes `chunk` tokens of all heads of K (y = 0) or V; D / 16 lanes a row.
 template <int D, bool BF>
 __global__ void __launch_bounds__(kThreads) prompt_append_kernel(const AppendArgs a) {
-    constexpr int L = D / 8;  // lanes of a row
-    __shared__ uint64_t dst[kMaxChunk];  // slot of head 0 of each token, or ~0
+    constexpr int L = D / kE;
+    constexpr uint32_t R = kThreads / L;  // rows of the block at a time
+    __shared__ uint64_t dst[kMaxChunk];   // slot of head 0 of each token, or ~0
     const uint32_t t0 = blockIdx.x * a.chunk, n_tok = min(a.chunk, a.tokens - t0);
+    const uint32_t rows = n_tok * a.heads;
+    const int lane = threadIdx.x % L;
+    const bool is_v = blockIdx.y;
+    const void* src = is_v ? a.src[1] : a.src[0];
+    const uint64_t ts = is_v ? a.ts[1] : a.ts[0], hs = is_v ? a.hs[1] : a.hs[0];
+    uint8_t* arena = is_v ? a.codes[1] : a.codes[0];
+    float* scales = is_v ? a.scales[1] : a.scales[0];
     pdl_wait_primary();
     int bad = 0;
     for (uint32_t b = threadIdx.x; b < a.branches; b += kThreads)
@@ -86,38 +188,74 @@ __global__ void __launch_bounds__(kThreads) prompt_append_kernel(const AppendArg
         dst[threadIdx.x] = d;
     }
     __syncthreads();
-    const uint32_t rows = 2 * n_tok * a.heads;
-    const int lane = threadIdx.x % L;
+    // R rows further: so many tokens and heads, the place in the source and the head's in the arena with them
+    const uint32_t step_tok = R / a.heads, step_head = R % a.heads;
+    const uint64_t step_from = step_tok * ts + step_head * hs, wrap_from = ts - a.heads * hs;
+    const uint64_t step_row = (uint64_t)step_head * a.capacity, wrap_row = (uint64_t)a.heads * a.capacity;
+    uint32_t tok = threadIdx.x / L / a.heads, head = threadIdx.x / L % a.heads;
+    uint64_t next_from = (uint64_t)(t0 + tok) * ts + head * hs + kE * lane, next_row = (uint64_t)head * a.capacity;
     bool finite = true;
-    for (uint32_t r = threadIdx.x / L; r < (rows + kThreads / L - 1) / (kThreads / L) * (kThreads / L); r += kThreads / L) {
-        const bool in = r < rows;
-        const uint32_t kv = in ? r / (n_tok * a.heads) : 0u, i = in ? r - kv * n_tok * a.heads : 0u;
-        const uint32_t tok = i / a.heads, head = i - tok * a.heads;
-        const uint64_t base = dst[tok];
-        const bool on = in && base != ~0ull;
-        float v[8];
+    for (uint32_t r0 = 0; r0 < rows; r0 += kRows * R) {  // the same number of turns for all of the block
+        Raw<BF> raw[kRows];
+        uint64_t slot[kRows], from[kRows];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = 0.f;
-        if (on) load_row8<BF>(a.src[kv], (uint64_t)(t0 + tok) * a.ts[kv] + head * a.hs[kv] + 8 * lane, a.vec, v);
-        float m = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            finite = finite && isfinite(v[k]);
-            m = fmaxf(m, fabsf(v[k]));
+        for (int u = 0; u < kRows; ++u) {
+            slot[u] = tok < n_tok ? dst[tok] : ~0ull;
+            from[u] = next_from;
+            raw[u] = Raw<BF>{};
+            if (slot[u] != ~0ull) {
+                slot[u] += next_row;
+                raw[u] = load_raw<BF>(src, next_from, a.vec);
+            }
+            tok += step_tok;
+            head += step_head;
+            next_from += step_from;
+            next_row += step_row;
+            if (head >= a.heads) {
+                head -= a.heads;
+                ++tok;
+                next_from += wrap_from;
+                next_row -= wrap_row;
+            }
         }
 #pragma unroll
-        for (int o = L / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float s = fmaxf(__fdiv_rn(m, 127.f), 1e-12f);
-        uint32_t w[2] = {0u, 0u};
+        for (int u = 0; u < kRows; ++u) {
+            float v[kE], m = largest<BF>(raw[u]);
+            unpack<BF>(raw[u], v);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int q = max(-127, min(127, __float2int_rn(__fdiv_rn(v[k], s))));
-            w[k / 4] |= (uint32_t)(q & 0xff) << (8 * (k % 4));
-        }
-        if (on) {
-            const uint64_t slot = base + (uint64_t)head * a.capacity;
-            *reinterpret_cast<uint2*>(a.codes[kv] + slot * D + 8 * lane) = make_uint2(w[0], w[1]);
-            if (lane == 0) a.scales[kv][slot] = s;
+            for (int o = L / 2; o; o >>= 1) {
+                const float y = __shfl_xor_sync(0xffffffffu, m, o);
+                asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(y));
+            }
+            float s = fmaxf(over_127(m), 1e-12f);
+            const float y = __frcp_rn(s);
+            const uint64_t y2 = f2_pack(y, y), s2 = f2_pack(-s, -s), up = f2_pack(12582912.f, 12582912.f);
+            uint32_t w[kE / 4];
+#pragma unroll
+            for (int k = 0; k < kE; k += 4) {
+                float c[4];
+#pragma unroll
+                for (int h = 0; h < 4; h += 2) {
+                    const uint64_t x = f2_pack(v[k + h], v[k + h + 1]);
+                    uint64_t q = f2_mul(x, y2);
+                    q = f2_fma(f2_fma(q, s2, x), y2, q);
+                    q = f2_fma(f2_fma(q, s2, x), y2, q);
+                    f2_unpack(f2_add(q, up), c[h], c[h + 1]);
+                }
+                w[k / 4] = __byte_perm(__byte_perm(__float_as_uint(c[0]), __float_as_uint(c[1]), 0x0040),
+                                       __byte_perm(__float_as_uint(c[2]), __float_as_uint(c[3]), 0x0040), 0x5410);
+            }
+            uint4 codes = make_uint4(w[0], w[1], w[2], w[3]);
+            if (!isfinite(m)) {  // all the row's lanes
+                const Divided d = divided<D, BF>(src, from[u], a.vec);
+                codes = d.codes;
+                s = d.s;
+                finite = finite && d.finite;
+            }
+            if (slot[u] != ~0ull) {
+                *reinterpret_cast<uint4*>(arena + slot[u] * D + kE * lane) = codes;
+                if (lane == 0) scales[slot[u]] = s;
+            }
         }
     }
     if (!finite && a.status) atomicOr(a.status, PP_DEV_NONFINITE_INPUT);
@@ -145,8 +283,12 @@ cudaError_t launch_prompt_append(const PromptAppendLaunch& P, cudaStream_t strea
     a.capacity = P.arena->capacity;
     a.vec = P.vec;
     a.status = P.status;
-    a.chunk = 4;
-    const dim3 grid((P.tokens + a.chunk - 1) / a.chunk);
+    // About 24 CTAs an SM where the prompts are long, at least one turn of rows each where they are short.
+    const uint32_t turn = kRows * kThreads / (P.arena->head_dim / kE);
+    uint32_t chunk = P.tokens / (12 * P.num_sms);
+    chunk = chunk > (turn + a.heads - 1) / a.heads ? chunk : (turn + a.heads - 1) / a.heads;
+    a.chunk = chunk < kMaxChunk ? chunk : kMaxChunk;
+    const dim3 grid((P.tokens + a.chunk - 1) / a.chunk, 2);
     if (P.arena->head_dim == 128)
         return P.bf16 ? launch_pdl(prompt_append_kernel<128, true>, grid, dim3(kThreads), stream, a)
                       : launch_pdl(prompt_append_kernel<128, false>, grid, dim3(kThreads), stream, a);

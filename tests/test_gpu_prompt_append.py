@@ -155,3 +155,20 @@ def test_captured_replay_takes_new_lengths(pp, cuda):
         starts.copy_(starts_of(lens, cuda)), offsets.copy_(torch.tensor(offs, device=cuda))
         graph.replay()
         assert same(arena, expected(pp, arena, k, v, lens, offs))
+
+
+def test_every_mantissa_of_a_maximum(pp, cuda):
+    """All 2^23 maxima between 1 and 2, each with 63 elements on or within two units of half-integer quotients."""
+    n, d = 2**23, 64
+    top = torch.arange(2**23, dtype=torch.int32, device=cuda).add_(0x3F800000).view(torch.float32)
+    g = torch.Generator(device=cuda)
+    g.manual_seed(12)
+    x = torch.randint(-127, 127, (n, 1, d), device=cuda, generator=g).float().add_(0.5)
+    x.mul_((top / torch.full_like(top, 127.0))[:, None, None])
+    x.view(torch.int32).add_(torch.randint(-2, 3, (n, 1, d), device=cuda, generator=g, dtype=torch.int32))
+    x.clamp_(min=-top[:, None, None], max=top[:, None, None])
+    x[:, 0, 0] = top
+    arena = pp.kv_cache.Int8KvArena.zeros(1, 1, d, n, cuda)
+    arena.append_prompt(x, x, starts_of([n], cuda), torch.zeros(1, dtype=torch.int32, device=cuda))
+    codes, scales = pp.int8_kv_ops.quantize(x.view(1, n, d))
+    assert torch.equal(arena.k_scale, scales) and torch.equal(arena.k, codes) and torch.equal(arena.v, codes)
