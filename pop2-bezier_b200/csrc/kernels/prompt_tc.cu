@@ -50,6 +50,9 @@ struct TcCfg {
     static constexpr uint32_t STAGES = D == 128 ? 5 : 8;  // K and V tiles in flight
     static constexpr uint32_t SMEM = 1024 + 2 * TILE + STAGES * TILE;
     static constexpr uint32_t S_COL = 0, O_COL = 256;     // tile t: + 128 t, + D t
+    // Registers of a thread of the softmax and of the others (2 x + y = 3 * 168): the
+    // products' thread keeps 32 descriptors at head_dim 128, half of them at 64.
+    static constexpr int R_SOFTMAX = D == 128 ? 208 : 216, R_OTHER = D == 128 ? 88 : 72;
 };
 
 struct Item {
@@ -234,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_OTHER));
         if (warp == 9 && lane == 0) {
             // ------------------------------------------------ items and loads
             PromptHeader* hdr = reinterpret_cast<PromptHeader*>(a.ws);
@@ -475,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::R_SOFTMAX));
         // ------------------------------------------------------- the softmax
         const uint32_t t = warp >> 2, r = threadIdx.x & 127, wl = (warp & 3) * 32;
         const uint32_t s_addr = tmem + (wl << 16) + C::S_COL + 128 * t, o_addr = tmem + (wl << 16) + C::O_COL + D * t;
@@ -492,17 +495,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t it = 0;; ++it) {
             const uint32_t slot = it & 1;
             if (!wait(&sh.item_full[slot], (it >> 1) & 1)) break;
-            const PromptEntry e = sh.item[slot].e;
-            const uint32_t head = sh.item[slot].head, valid = sh.item[slot].valid;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.item_empty[slot]);
-            if (!valid) break;
-            const Geo g = geometry_of(a, e, t);
-            const uint32_t n = g.n, live_rows = g.live;
-            const uint32_t token = g.tok + r / a.group;
-            const bool live = r < live_rows;
-            const uint32_t lim = live ? min(e.kv_end, prompt_visible(e, token, a.causal)) : 0u;
-            if (!live_rows) continue;
+            // The item stays in shared memory until this warp is done with it: its fields are read again after the
+            // key tiles, whose loop needs the registers.
+            const PromptEntry& e = sh.item[slot].e;
+            if (!sh.item[slot].valid) break;
+            uint32_t n, first, lim;
+            {
+                const Geo g = geometry_of(a, e, t);
+                n = g.n;
+                first = g.first;
+                // a row that does not exist masks nothing: masks cost time, and nobody looks at it
+                lim = r < g.live ? min(e.kv_end, prompt_visible(e, g.tok + r / a.group, a.causal)) : 0xffffffffu;
+                if (!g.live) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.item_empty[slot]);
+                    continue;
+                }
+            }
             float m = -CUDART_INF_F, z = 0.f;
             bool ok = true;
             for (uint32_t j = 0; j < n; ++j) {
@@ -512,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_ld32(reinterpret_cast<uint32_t(&)[32]>(s[32 * c]), s_addr + 32 * c);
                 tmem_wait_ld();
-                const uint32_t n0 = g.first + j * kPromptKeyTile;
+                const uint32_t n0 = first + j * kPromptKeyTile;
                 const uint32_t see = lim > n0 ? lim - n0 : 0u;  // of this tile
                 if (__any_sync(0xffffffffu, see < kPromptKeyTile)) {
 #pragma unroll
@@ -582,6 +591,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!wait(&sh.o_full[t], o_use++ & 1)) break;
                 tc_fence_after();
             }
+            const Geo g = geometry_of(a, e, t);
+            const uint32_t head = sh.item[slot].head, live_rows = g.live;
+            const bool live = r < live_rows;
+            auto done_with_item = [&] {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.item_empty[slot]);
+            };
             float f0 = 1.f, f1 = 0.f;  // of this tile's output and of its other half's
             if (g.halves) {
                 if (t) {
@@ -590,6 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.half_full);
                     if (!wait(&sh.half_empty, half_use++ & 1)) break;
+                    done_with_item();
                     continue;
                 }
                 if (!wait(&sh.half_full, half_use++ & 1)) break;
@@ -739,6 +756,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) atomicSub(&sh.redoing, 1);
             }
+            done_with_item();
             tc_fence_before();  // O has been read before the next item's first product may start (p_full)
         }
     }
