@@ -132,8 +132,7 @@ struct AttnLaunch {
 //   PromptHeader                            @ 0
 //   seq_base  u32 [sequences + 1]     first uncut entry of each sequence
 //   entries   PromptEntry [max_entries]     longest first
-//   counters  u32 [max_ctas * 4]      finished splits per cut item and 64 rows
-//                                     (zero between calls)
+//   cuts      u32 [max_ctas]                first piece of each cut entry
 //   acc       f32 [slots][slot_rows][head_dim]   partials of cut items
 //   ml        f32 [slots][slot_rows][2]          their maximum (log2 units), sum
 // An entry is cut only when its keys are more than its share of all the work,
@@ -143,7 +142,8 @@ struct PromptHeader {
     uint32_t n_entries;
     uint32_t n_items;  // entries * kv_heads
     uint32_t next;     // next item to hand out beyond the grid's first ones (zero between calls)
-    uint32_t pad[5];
+    uint32_t n_cuts;   // entries cut along their keys
+    uint32_t pad[4];
 };
 
 struct PromptEntry {
@@ -153,12 +153,11 @@ struct PromptEntry {
     uint32_t kv_begin, kv_end;    // keys of this piece, within the sequence
     uint32_t split, n_splits;     // which piece of how many
     uint32_t slot0;               // slot of piece s and head h: (slot0 + s) * kv_heads + h
-    uint32_t counter;             // counters of head h: 4 * (counter * kv_heads + h)
-    uint32_t pad;
+    uint32_t pad[2];
 };
 
 struct PromptWsLayout {
-    size_t seq_base, entries, counters, acc, ml, total;
+    size_t seq_base, entries, cuts, acc, ml, total;
     uint32_t max_entries, max_slots, slot_rows, max_ctas;
 };
 
@@ -175,8 +174,8 @@ inline PromptWsLayout prompt_ws_layout(uint32_t sequences, uint32_t q_tokens, ui
     off = align_up(off + 4ull * (sequences + 1ull), 256);
     l.entries = off;
     off = align_up(off + sizeof(PromptEntry) * (size_t)l.max_entries, 256);
-    l.counters = off;
-    off = align_up(off + 16ull * max_ctas, 256);
+    l.cuts = off;
+    off = align_up(off + 4ull * max_ctas, 256);
     l.acc = off;
     off = align_up(off + 4ull * l.max_slots * l.slot_rows * head_dim, 256);
     l.ml = off;
@@ -202,6 +201,8 @@ cudaError_t configure_prompt_kernels();
 int32_t check_arena(const PpKvArena* a, const char* what);
 cudaError_t launch_prompt_plan(const PromptLaunch& L, cudaStream_t stream);
 cudaError_t launch_prompt_rows(const PromptLaunch& L, cudaStream_t stream);
+uint32_t prompt_uncut_keys();
+cudaError_t launch_prompt_merge(const PromptLaunch& L, cudaStream_t stream);
 cudaError_t configure_prompt_tc_kernels();
 cudaError_t launch_prompt_tc(const PromptLaunch& L, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                              cudaStream_t stream);

@@ -138,8 +138,11 @@ int32_t pp_b200_prompt_attention(const PpPrompt* prompt, const uint32_t* q_start
     }
     if (!(L.g.flags & PP_ATTN_PLAN_READY) && (s = pp::cuda_status(pp::launch_prompt_plan(L, st), "prompt plan launch")))
         return s;
-    if (!tc) return pp::cuda_status(pp::launch_prompt_rows(L, st), "prompt attention launch");
-    return pp::cuda_status(pp::launch_prompt_tc(L, map_q, map_k, map_v, st), "prompt attention launch");
+    s = pp::cuda_status(tc ? pp::launch_prompt_tc(L, map_q, map_k, map_v, st) : pp::launch_prompt_rows(L, st),
+                        "prompt attention launch");
+    // no entry of so few keys is cut (prompt.cu)
+    if (s || L.g.kv_tokens <= pp::prompt_uncut_keys()) return s;
+    return pp::cuda_status(pp::launch_prompt_merge(L, st), "prompt merge launch");
 }
 
 int32_t pp_b200_prompt_append(const PpKvArena* arena, const void* k, const void* v, int32_t dtype, uint32_t tokens,

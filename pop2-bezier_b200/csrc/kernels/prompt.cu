@@ -15,15 +15,14 @@ namespace {
 // of length), because the attention CTAs take items in this order as they
 // become free: the last ones taken are the shortest.  Where the whole batch has
 // fewer steps than it takes to keep every CTA busy with whole entries, an entry
-// of more than one and a half times its share is cut into equal pieces along
-// the keys; below that, the merge and the uneven last round cost what the cut
-// gains.
+// of more than one and a half times its share, and of at least kCutSteps, is cut
+// into equal pieces along the keys; below that, the partials, the merge and the
+// uneven last round cost what the cut gains (the merge launch and the partials take
+// about as long as four steps).
 constexpr int kPlanThreads = 1024;
 constexpr uint32_t kClasses = 64;
 constexpr uint32_t kBaseMax = 2048;  // sequences whose first entries are kept in shared memory
-#ifndef PP_PROMPT_MIN_SHARE
-#define PP_PROMPT_MIN_SHARE 2
-#endif
+constexpr uint32_t kCutSteps = 12;
 
 struct PlanArgs {
     const uint32_t* q_starts;
@@ -94,7 +93,7 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
     PromptHeader* hdr = reinterpret_cast<PromptHeader*>(a.ws);
     uint32_t* seq_base = a.sequences <= kBaseMax ? base_s : reinterpret_cast<uint32_t*>(a.ws + a.l.seq_base);
     PromptEntry* entries = reinterpret_cast<PromptEntry*>(a.ws + a.l.entries);
-    uint32_t* counters = reinterpret_cast<uint32_t*>(a.ws + a.l.counters);
+    uint32_t* cut_list = reinterpret_cast<uint32_t*>(a.ws + a.l.cuts);
     if (t == 0) longest = slots = cuts = 0;
     if (t < kClasses) hist[t] = 0;
     // launched as a programmatic dependent: the kernels before may still read
@@ -102,7 +101,6 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
     // start now; it waits for this kernel before it reads the plan.
     pdl_wait_primary();
     pdl_launch_dependents();
-    for (uint32_t i = t; i < 4 * a.l.max_ctas; i += kPlanThreads) counters[i] = 0;
     int bad = 0;
     uint32_t n = 0;
     for (uint32_t b0 = 0; b0 < a.sequences; b0 += kPlanThreads) {
@@ -150,11 +148,11 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
     for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
     all *= a.kv_heads;
     const unsigned long long share = (all + a.l.max_ctas - 1) / a.l.max_ctas;
-    const uint32_t limit = (uint32_t)max((unsigned long long)PP_PROMPT_MIN_SHARE, min(share + share / 2, 0x7fffffffull));
-    const uint32_t most = min(longest, limit);  // steps of the longest piece
+    const uint32_t limit = (uint32_t)max(2ull, min(share + share / 2, 0x7fffffffull));
+    const uint32_t most = longest;
     // pieces of an entry and the class of their length (steps < 2^25, so the product fits)
     auto cut = [&](const Whole& w, uint32_t& pieces) {
-        pieces = (w.steps + limit - 1) / limit;
+        pieces = w.steps < kCutSteps ? 1u : (w.steps + limit - 1) / limit;
         const uint32_t len = (w.steps + pieces - 1) / pieces;
         return kClasses - 1 - (len - 1) * kClasses / most;
     };
@@ -186,10 +184,10 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
         const uint32_t at = atomicAdd(&cursor[cut(w, pieces)], pieces);
         PromptEntry p = w.p;
         p.n_splits = pieces;
-        p.slot0 = p.counter = p.pad = 0;
+        p.slot0 = p.pad[0] = p.pad[1] = 0;
         if (pieces > 1) {
             p.slot0 = atomicAdd(&slots, pieces);
-            p.counter = atomicAdd(&cuts, 1u);
+            cut_list[atomicAdd(&cuts, 1u)] = at;
         }
         const uint32_t end = p.kv_end;
         for (uint32_t s = 0; s < pieces; ++s) {
@@ -200,6 +198,8 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
             entries[at + s] = p;
         }
     }
+    __syncthreads();
+    if (t == 0) hdr->n_cuts = cuts;
 }
 
 // ------------------------------------------------------ the CUDA-core kernel
@@ -253,13 +253,12 @@ __global__ void __launch_bounds__(kRowsThreads) prompt_rows_kernel(const PromptA
     float* sk = sq + 64 * C::LD;
     float* sv = sk + 64 * C::LD;
     float* sp = sv + 64 * D;
-    __shared__ uint32_t s_next, s_last;
+    __shared__ uint32_t s_next;
     const int t = threadIdx.x, tx = t & 15, ty = t >> 4;
     PromptHeader* hdr = reinterpret_cast<PromptHeader*>(a.ws);
     const PromptEntry* entries = reinterpret_cast<const PromptEntry*>(a.ws + a.l.entries);
     float* acc_ws = reinterpret_cast<float*>(a.ws + a.l.acc);
     float* ml_ws = reinterpret_cast<float*>(a.ws + a.l.ml);
-    uint32_t* counters = reinterpret_cast<uint32_t*>(a.ws + a.l.counters);
     pdl_wait_primary();
     const uint32_t units = hdr->n_items * 4, n_entries = hdr->n_entries;
     uint32_t unit = blockIdx.x;
@@ -426,7 +425,7 @@ __global__ void __launch_bounds__(kRowsThreads) prompt_rows_kernel(const PromptA
                     write_row(i, o, z[i]);
                 }
             } else {
-                // partial of this piece; the CTA that brings the last one merges them in the order of the pieces
+                // partial of this piece, for prompt_merge_kernel
                 const uint32_t srow = tile * kPromptTileRows + row0;
                 auto slot_row = [&](uint32_t s, uint32_t r) {
                     return (uint64_t)((e.slot0 + s) * a.kv_heads + head) * a.l.slot_rows + srow + r;
@@ -444,38 +443,6 @@ __global__ void __launch_bounds__(kRowsThreads) prompt_rows_kernel(const PromptA
                         ml_ws[2 * at + 1] = z[i];
                     }
                 }
-                uint32_t* cnt = counters + 4 * (e.counter * a.kv_heads + head) + sub;
-                __threadfence();
-                __syncthreads();
-                if (t == 0) s_last = atomicAdd(cnt, 1u) + 1 == e.n_splits;
-                __syncthreads();
-                if (s_last) {
-                    __threadfence();
-                    if (t == 0) *cnt = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (!live(4 * ty + i)) continue;
-                        float top = -CUDART_INF_F, sum = 0.f, o[4 * H] = {};
-                        for (uint32_t s = 0; s < e.n_splits; ++s)
-                            top = fmaxf(top, __ldcg(ml_ws + 2 * slot_row(s, 4 * ty + i)));
-                        const float ref = top == -CUDART_INF_F ? 0.f : top;
-                        for (uint32_t s = 0; s < e.n_splits; ++s) {
-                            const uint64_t at = slot_row(s, 4 * ty + i);
-                            const float zs = __ldcg(ml_ws + 2 * at + 1), f = exp2f(__ldcg(ml_ws + 2 * at) - ref);
-                            if (zs == 0.f) continue;  // this row saw nothing of the piece
-                            sum += zs * f;
-#pragma unroll
-                            for (int h = 0; h < H; ++h) {
-                                const float4 x = __ldcg(reinterpret_cast<const float4*>(acc_ws + at * D + 64 * h + 4 * tx));
-                                o[4 * h] += x.x * f;
-                                o[4 * h + 1] += x.y * f;
-                                o[4 * h + 2] += x.z * f;
-                                o[4 * h + 3] += x.w * f;
-                            }
-                        }
-                        write_row(i, o, sum);
-                    }
-                }
             }
         }
         __syncthreads();
@@ -486,6 +453,77 @@ __global__ void __launch_bounds__(kRowsThreads) prompt_rows_kernel(const PromptA
         }
         __syncthreads();
         unit = s_next;
+    }
+}
+
+// --------------------------------------------------- the pieces of cut rows
+//
+// A warp merges a row: out = sum_s 2^(m_s - m) acc_s / sum_s 2^(m_s - m) z_s over
+// its pieces in their order, whoever finished last.  Merging inside the attention
+// kernels, by the CTA that brings an entry's last piece, took 17 to 33 thousand
+// cycles (one CTA's loads, and code that only it runs); spread over the GPU this
+// takes two or three microseconds, and one where nothing is cut.
+constexpr int kMergeWarps = 8;
+
+template <int D, bool BF>
+__global__ void __launch_bounds__(32 * kMergeWarps) prompt_merge_kernel(const __grid_constant__ PromptArgs a) {
+    constexpr int C = D / 32;  // channels of a lane
+    const uint32_t lane = threadIdx.x & 31;
+    const PromptHeader* hdr = reinterpret_cast<const PromptHeader*>(a.ws);
+    const PromptEntry* entries = reinterpret_cast<const PromptEntry*>(a.ws + a.l.entries);
+    const uint32_t* cuts = reinterpret_cast<const uint32_t*>(a.ws + a.l.cuts);
+    const float* acc = reinterpret_cast<const float*>(a.ws + a.l.acc);
+    const float* ml = reinterpret_cast<const float*>(a.ws + a.l.ml);
+    pdl_wait_primary();
+    const uint32_t groups = hdr->n_cuts * a.kv_heads, rows = a.l.slot_rows;
+    for (uint64_t i = (uint64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5); i < (uint64_t)groups * rows;
+         i += (uint64_t)gridDim.x * kMergeWarps) {
+        const uint32_t row = (uint32_t)(i % rows), head = (uint32_t)(i / rows) % a.kv_heads;
+        const PromptEntry e = entries[cuts[(uint32_t)(i / rows) / a.kv_heads]];
+        const uint32_t r = row % kPromptTileRows;  // of its tile
+        const uint32_t token = e.tok0 + row / kPromptTileRows * a.tpt + r / a.group;
+        if (r >= a.tpt * a.group || token >= e.nq) continue;
+        const uint64_t first = ((uint64_t)e.slot0 * a.kv_heads + head) * rows + row, step = (uint64_t)a.kv_heads * rows;
+        float m = -CUDART_INF_F, z = 0.f, o[C];
+        for (uint32_t s = lane; s < e.n_splits; s += 32) m = fmaxf(m, ml[2 * (first + s * step)]);
+#pragma unroll
+        for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+        const float ref = m == -CUDART_INF_F ? 0.f : m;
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[c] = 0.f;
+        for (uint32_t s0 = 0; s0 < e.n_splits; s0 += 32) {
+            float w = 0.f, zs = 0.f;
+            if (s0 + lane < e.n_splits) {
+                const float2 mz = *reinterpret_cast<const float2*>(ml + 2 * (first + (s0 + lane) * step));
+                if (mz.y != 0.f) w = exp2f(mz.x - ref);  // 0: the row saw nothing of this piece
+                zs = mz.y * w;
+            }
+            const uint32_t n = min(32u, e.n_splits - s0);
+#pragma unroll 4
+            for (uint32_t s = 0; s < n; ++s) {
+                float x[C];
+#pragma unroll
+                for (int c = 0; c < C; ++c) x[c] = acc[(first + (s0 + s) * step) * D + C * lane + c];
+                const float ws = __shfl_sync(0xffffffffu, w, s);
+                z += __shfl_sync(0xffffffffu, zs, s);
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+                    if (ws != 0.f) o[c] += x[c] * ws;
+            }
+        }
+        const uint64_t at = ((uint64_t)(e.q0 + token) * a.heads + head * a.group + r % a.group) * D + C * lane;
+        const float inv = z == 0.f ? CUDART_NAN_F : 1.f / z;  // a row that sees no key
+        bool bad = false;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            o[c] *= inv;
+            bad = bad || !(o[c] * 0.f == 0.f);
+            if constexpr (BF) reinterpret_cast<__nv_bfloat16*>(a.out)[at + c] = __float2bfloat16_rn(o[c]);
+            else reinterpret_cast<float*>(a.out)[at + c] = o[c];
+        }
+        if constexpr (BF) {
+            if (a.vec && __any_sync(0xffffffffu, bad) && z != 0.f) redo_row<D>(a, e, head, token, r % a.group);
+        }
     }
 }
 
@@ -571,6 +609,20 @@ cudaError_t launch_prompt_rows(const PromptLaunch& L, cudaStream_t stream) {
         return bf ? launch_rows<64, true>(a, 3 * L.layout.max_ctas, stream)
                   : launch_rows<64, false>(a, 3 * L.layout.max_ctas, stream);
     return bf ? launch_rows<128, true>(a, L.layout.max_ctas, stream) : launch_rows<128, false>(a, L.layout.max_ctas, stream);
+}
+
+// An entry takes no more steps than its keys have tiles.
+uint32_t prompt_uncut_keys() { return (kCutSteps - 1) * kPromptKeyTile; }
+
+cudaError_t launch_prompt_merge(const PromptLaunch& L, cudaStream_t stream) {
+    const PromptArgs a = prompt_args(L);
+    const dim3 grid(2 * L.num_sms), block(32 * kMergeWarps);
+    const bool bf = L.g.dtype == PP_DTYPE_BF16;
+    if (L.g.head_dim == 64)
+        return bf ? launch_pdl(prompt_merge_kernel<64, true>, grid, block, stream, a)
+                  : launch_pdl(prompt_merge_kernel<64, false>, grid, block, stream, a);
+    return bf ? launch_pdl(prompt_merge_kernel<128, true>, grid, block, stream, a)
+              : launch_pdl(prompt_merge_kernel<128, false>, grid, block, stream, a);
 }
 
 }  // namespace pp

@@ -1,5 +1,5 @@
-// Shared by the prompt attention kernels: the work list in the workspace and
-// the merge of a row that was cut along its keys.
+// Shared by the prompt attention kernels: the work list in the workspace, and a
+// row computed by itself.
 //
 // A work item is one K/V head of one entry; an entry is 256 consecutive query
 // rows of one sequence against a range of its keys.  The G = heads / kv_heads
@@ -43,10 +43,56 @@ __device__ __forceinline__ uint32_t prompt_visible(const PromptEntry& e, uint32_
     return v > e.nq ? (uint32_t)min((uint64_t)e.nk, v - e.nq) : 0u;
 }
 
-__device__ __forceinline__ uint32_t ld_acquire(const uint32_t* p) {
-    uint32_t v;
-    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
+// One row by one warp from the keys it sees and nothing else: what a tile does with
+// masks does not hold where a masked value is not finite.  bf16 rows on 16-byte
+// boundaries.
+template <int D>
+__device__ __noinline__ void redo_row(const PromptArgs& a, const PromptEntry& e, uint32_t head, uint32_t token,
+                                      uint32_t g) {
+    constexpr int E = D / 32;
+    const int lane = threadIdx.x & 31;
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (uint64_t)(e.q0 + token) * a.q_ts +
+                        (uint64_t)(head * a.group + g) * a.q_hs;
+    const uint32_t end = prompt_visible(e, token, a.causal);
+    float m = -__int_as_float(0x7f800000), z = 0.f, acc[E];
+#pragma unroll
+    for (int c = 0; c < E; ++c) acc[c] = 0.f;
+    for (uint32_t n0 = 0; n0 < end; n0 += 32) {
+        float s = -__int_as_float(0x7f800000);
+        if (n0 + lane < end) {
+            const uint16_t* k = reinterpret_cast<const uint16_t*>(a.k) + ((uint64_t)e.k0 + n0 + lane) * a.k_ts +
+                                (uint64_t)head * a.k_hs;
+            float dot = 0.f;
+            for (int c = 0; c < D; c += 2) {
+                const uint32_t x = *reinterpret_cast<const uint32_t*>(q + c), y = *reinterpret_cast<const uint32_t*>(k + c);
+                dot = fmaf(bf16_lo_to_f32(x), bf16_lo_to_f32(y), dot);
+                dot = fmaf(bf16_hi_to_f32(x), bf16_hi_to_f32(y), dot);
+            }
+            s = dot * a.scale_log2;
+        }
+        float top = s;
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float mn = fmaxf(m, top), ref = mn == -__int_as_float(0x7f800000) ? 0.f : mn;
+        const float f = exp2f(m - ref), p = exp2f(s - ref);
+        float sum = p;
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        z = z * f + sum;
+        m = mn;
+#pragma unroll
+        for (int c = 0; c < E; ++c) acc[c] *= f;
+        const uint32_t cnt = min(32u, end - n0);
+        for (uint32_t i = 0; i < cnt; ++i) {
+            const float pi = __shfl_sync(0xffffffffu, p, i);
+            const uint16_t* v = reinterpret_cast<const uint16_t*>(a.v) + ((uint64_t)e.k0 + n0 + i) * a.v_ts +
+                                (uint64_t)head * a.v_hs;
+#pragma unroll
+            for (int c = 0; c < E; ++c) acc[c] = fmaf(pi, bf16_lo_to_f32(v[lane + 32 * c]), acc[c]);
+        }
+    }
+    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) +
+                         ((uint64_t)(e.q0 + token) * a.heads + head * a.group + g) * D;
+#pragma unroll
+    for (int c = 0; c < E; ++c) out[lane + 32 * c] = __float2bfloat16_rn(acc[c] / z);
 }
 
 }  // namespace pp

@@ -65,13 +65,11 @@ struct Shared {
     uint64_t q_full[2], q_empty[2];
     uint64_t s_full[2], p_full[2], o_full[2];
     uint64_t item_full[2], item_empty[2];
-    uint64_t group[2];  // a tile's four softmax warps meet
     uint64_t drain;
     Item item[2];
     uint32_t tmem;
     int abort;
     int redoing;       // warps that compute rows again: the others wait for them without a limit of their own
-    uint32_t last[2];  // of a tile: this CTA brought the last piece
     uint64_t half_full, half_empty;  // the second half of a shared tile is there, has been merged
     float2 half[128];                // its maximum and sum
 };
@@ -118,56 +116,6 @@ __device__ __forceinline__ void st_global_v8(float* p, const uint32_t* v) {
                  : "memory");
 }
 
-// A row again, by one warp, from the keys it sees and nothing else (see the top).
-template <int D>
-__device__ __noinline__ void redo_row(const PromptArgs& a, const PromptEntry& e, uint32_t head, uint32_t token,
-                                      uint32_t g) {
-    constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31;
-    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (uint64_t)(e.q0 + token) * a.q_ts +
-                        (uint64_t)(head * a.group + g) * a.q_hs;
-    const uint32_t end = prompt_visible(e, token, a.causal);
-    float m = -CUDART_INF_F, z = 0.f, acc[E];
-#pragma unroll
-    for (int c = 0; c < E; ++c) acc[c] = 0.f;
-    for (uint32_t n0 = 0; n0 < end; n0 += 32) {
-        float s = -CUDART_INF_F;
-        if (n0 + lane < end) {
-            const uint16_t* k = reinterpret_cast<const uint16_t*>(a.k) + ((uint64_t)e.k0 + n0 + lane) * a.k_ts +
-                                (uint64_t)head * a.k_hs;
-            float dot = 0.f;
-            for (int c = 0; c < D; c += 2) {
-                const uint32_t x = *reinterpret_cast<const uint32_t*>(q + c), y = *reinterpret_cast<const uint32_t*>(k + c);
-                dot = fmaf(bf16_lo_to_f32(x), bf16_lo_to_f32(y), dot);
-                dot = fmaf(bf16_hi_to_f32(x), bf16_hi_to_f32(y), dot);
-            }
-            s = dot * a.scale_log2;
-        }
-        float top = s;
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float mn = fmaxf(m, top), ref = mn == -CUDART_INF_F ? 0.f : mn;
-        const float f = exp2f(m - ref), p = exp2f(s - ref);
-        float sum = p;
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        z = z * f + sum;
-        m = mn;
-#pragma unroll
-        for (int c = 0; c < E; ++c) acc[c] *= f;
-        const uint32_t cnt = min(32u, end - n0);
-        for (uint32_t i = 0; i < cnt; ++i) {
-            const float pi = __shfl_sync(0xffffffffu, p, i);
-            const uint16_t* v = reinterpret_cast<const uint16_t*>(a.v) + ((uint64_t)e.k0 + n0 + i) * a.v_ts +
-                                (uint64_t)head * a.v_hs;
-#pragma unroll
-            for (int c = 0; c < E; ++c) acc[c] = fmaf(pi, bf16_lo_to_f32(v[lane + 32 * c]), acc[c]);
-        }
-    }
-    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) +
-                         ((uint64_t)(e.q0 + token) * a.heads + head * a.group + g) * D;
-#pragma unroll
-    for (int c = 0; c < E; ++c) out[lane + 32 * c] = __float2bfloat16_rn(acc[c] / z);
-}
-
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ TcMaps maps) {
@@ -193,7 +141,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&sh.o_full[t], 1);
             mbar_init(&sh.item_full[t], 1);
             mbar_init(&sh.item_empty[t], 9);
-            mbar_init(&sh.group[t], 4);
         }
         mbar_init(&sh.drain, 1);
         mbar_init(&sh.half_full, 4);
@@ -210,6 +157,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
+    pdl_launch_dependents();  // the merge may be set up meanwhile; it waits for this kernel before it reads
     pdl_wait_primary();
 
     auto give_up = [&] {
@@ -485,13 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t scale2 = f2_pack(a.scale_log2, a.scale_log2);
         float* acc_ws = reinterpret_cast<float*>(a.ws + a.l.acc);
         float* ml_ws = reinterpret_cast<float*>(a.ws + a.l.ml);
-        uint32_t* counters = reinterpret_cast<uint32_t*>(a.ws + a.l.counters);
-        uint32_t s_use = 0, o_use = 0, group_use = 0, half_use = 0;
-        auto meet = [&]() -> bool {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.group[t]);
-            return wait(&sh.group[t], group_use++ & 1);
-        };
+        uint32_t s_use = 0, o_use = 0, half_use = 0;
         for (uint32_t it = 0;; ++it) {
             const uint32_t slot = it & 1;
             if (!wait(&sh.item_full[slot], (it >> 1) & 1)) break;
@@ -667,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 again = __ballot_sync(0xffffffffu, live && lim > 0 && !(chk == 0.f));
             } else {
-                // partial of this piece; the CTA that brings the last one merges them in the order of the pieces
+                // partial of this piece, for prompt_merge_kernel
                 auto slot_row = [&](uint32_t s, uint32_t row) {
                     return (uint64_t)((e.slot0 + s) * a.kv_heads + head) * a.l.slot_rows + t * kPromptTileRows + row;
                 };
@@ -682,65 +624,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 if (live) *reinterpret_cast<float2*>(ml_ws + 2 * at) = make_float2(m, z);
-                uint32_t* cnt = counters + 4 * (e.counter * a.kv_heads + head) + t;
-                __threadfence();
-                if (!meet()) break;
-                if (r == 0) sh.last[t] = atomicAdd(cnt, 1u) + 1 == e.n_splits;
-                if (!meet()) break;
-                if (sh.last[t]) {
-                    __threadfence();
-                    if (r == 0) *cnt = 0;
-                    // A warp merges its own 32 rows, all their loads of a piece in flight at once: lane l has
-                    // the weights of row l and 4 channels of every (D = 64: every other) row.
-                    constexpr int RPL = 128 / D;  // rows a load takes
-                    const uint32_t sub = lane / (D / 4), col = lane % (D / 4) * 4;
-                    float top = -CUDART_INF_F, sum = 0.f;
-                    if (live) {
-#pragma unroll 4
-                        for (uint32_t s = 0; s < e.n_splits; ++s) top = fmaxf(top, __ldcg(ml_ws + 2 * slot_row(s, r)));
-                    }
-                    const float ref = top == -CUDART_INF_F ? 0.f : top;
-                    float4 o[32 / RPL];
-#pragma unroll
-                    for (int i = 0; i < 32 / RPL; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (uint32_t s = 0; s < e.n_splits; ++s) {
-                        float w = 0.f;
-                        if (live) {
-                            const float2 mz = __ldcg(reinterpret_cast<const float2*>(ml_ws + 2 * slot_row(s, r)));
-                            if (mz.y != 0.f) w = exp2f(mz.x - ref);  // 0: the row saw nothing of this piece
-                            sum += mz.y * w;
-                        }
-                        const float* from = acc_ws + slot_row(s, warp_row) * D;
-#pragma unroll
-                        for (int i = 0; i < 32 / RPL; ++i) {
-                            const uint32_t row = i * RPL + sub;
-                            const float wr = __shfl_sync(0xffffffffu, w, row);
-                            if (warp_row + row < live_rows && wr != 0.f) {
-                                const float4 x = __ldcg(reinterpret_cast<const float4*>(from + row * D + col));
-                                o[i].x += x.x * wr;
-                                o[i].y += x.y * wr;
-                                o[i].z += x.z * wr;
-                                o[i].w += x.w * wr;
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 32 / RPL; ++i) {
-                        const uint32_t row = i * RPL + sub;
-                        const float inv = 1.f / __shfl_sync(0xffffffffu, sum, row);
-                        const float4 x = make_float4(o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv);
-                        const bool mine = warp_row + row < live_rows;
-                        if (mine)
-                            *reinterpret_cast<uint2*>(out_row(warp_row + row) + col) =
-                                make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
-                        const uint32_t bad =
-                            __ballot_sync(0xffffffffu, mine && !(x.x * 0.f + x.y * 0.f + x.z * 0.f + x.w * 0.f == 0.f));
-#pragma unroll
-                        for (int k = 0; k < RPL; ++k)
-                            if (bad >> (k * (D / 4)) & (uint32_t)((1ull << (D / 4)) - 1)) again |= 1u << (i * RPL + k);
-                    }
-                }
-                if (!meet()) break;  // sh.last has been read before the next item writes it
             }
             if (g.halves && lane == 0) {
                 tc_fence_before();
