@@ -260,12 +260,12 @@ __global__ void __launch_bounds__(kRowsThreads) prompt_rows_kernel(const PromptA
     float* acc_ws = reinterpret_cast<float*>(a.ws + a.l.acc);
     float* ml_ws = reinterpret_cast<float*>(a.ws + a.l.ml);
     pdl_wait_primary();
-    const uint32_t units = hdr->n_items * 4, n_entries = hdr->n_entries;
+    const uint32_t units = hdr->n_items * 4;
     uint32_t unit = blockIdx.x;
     while (unit < units) {
         const uint32_t item = unit >> 2, sub = unit & 3;
-        const uint32_t head = item / n_entries;
-        const PromptEntry e = entries[item - head * n_entries];
+        const uint32_t at = item / a.kv_heads, head = item - at * a.kv_heads;
+        const PromptEntry e = entries[at];
         const uint32_t tile = sub >> 1, row0 = (sub & 1) * kPromptSubRows;
         const uint32_t rows = min(a.tpt * a.group, row0 + kPromptSubRows);  // of the tile, up to this unit's end
         const uint32_t tile_tok = e.tok0 + tile * a.tpt;

@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ------------------------------------------------ items and loads
             PromptHeader* hdr = reinterpret_cast<PromptHeader*>(a.ws);
             const PromptEntry* entries = reinterpret_cast<const PromptEntry*>(a.ws + a.l.entries);
-            const uint32_t n_items = hdr->n_items, n_entries = hdr->n_entries;
+            const uint32_t n_items = hdr->n_items;
             const uint32_t q_bytes = a.group * a.tpt * 128 * (D / 64);
             uint32_t stage = 0, phase = 0, kv = 0, q_use0 = 0, q_use1 = 0, idx = blockIdx.x;
             bool ok = true;
@@ -225,8 +225,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive(&sh.item_full[slot]);
                     break;
                 }
-                const uint32_t head = idx / n_entries;
-                const PromptEntry e = entries[idx - head * n_entries];
+                const uint32_t at = idx / a.kv_heads, head = idx - at * a.kv_heads;
+                const PromptEntry e = entries[at];
                 item.e = e;
                 item.head = head;
                 mbar_arrive(&sh.item_full[slot]);
