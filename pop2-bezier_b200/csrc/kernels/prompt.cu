@@ -245,7 +245,7 @@ struct RowsCfg {
 };
 
 template <int D, bool BF>
-__global__ void __launch_bounds__(kRowsThreads) prompt_rows_kernel(const PromptArgs a) {
+__global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) prompt_rows_kernel(const PromptArgs a) {
     using C = RowsCfg<D>;
     constexpr int H = D / 64;  // channel groups of 4 a thread holds
     extern __shared__ __align__(16) float sm[];
@@ -367,20 +367,27 @@ __global__ void __launch_bounds__(kRowsThreads) prompt_rows_kernel(const PromptA
                 }
                 __syncwarp();  // the rows of a half-warp are its own
                 if (!masked) {
-#pragma unroll 4
-                    for (int n = 0; n < kBN; ++n) {
-                        ulonglong2 vv[H];
+#pragma unroll 2
+                    for (int n = 0; n < kBN; n += 4) {  // four keys' probabilities of a row in one load
+                        float4 p4[4];
 #pragma unroll
-                        for (int h = 0; h < H; ++h)
-                            vv[h] = *reinterpret_cast<const ulonglong2*>(sv + n * D + 64 * h + 4 * tx);
+                        for (int i = 0; i < 4; ++i)
+                            p4[i] = *reinterpret_cast<const float4*>(sp + (4 * ty + i) * (kBN + 4) + n);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float p = sp[(4 * ty + i) * (kBN + 4) + n];
-                            const uint64_t p2 = f2_pack(p, p);
+                        for (int u = 0; u < 4; ++u) {
+                            ulonglong2 vv[H];
 #pragma unroll
-                            for (int h = 0; h < H; ++h) {
-                                acc[i][2 * h] = f2_fma(p2, vv[h].x, acc[i][2 * h]);
-                                acc[i][2 * h + 1] = f2_fma(p2, vv[h].y, acc[i][2 * h + 1]);
+                            for (int h = 0; h < H; ++h)
+                                vv[h] = *reinterpret_cast<const ulonglong2*>(sv + (n + u) * D + 64 * h + 4 * tx);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float p = u == 0 ? p4[i].x : u == 1 ? p4[i].y : u == 2 ? p4[i].z : p4[i].w;
+                                const uint64_t p2 = f2_pack(p, p);
+#pragma unroll
+                                for (int h = 0; h < H; ++h) {
+                                    acc[i][2 * h] = f2_fma(p2, vv[h].x, acc[i][2 * h]);
+                                    acc[i][2 * h + 1] = f2_fma(p2, vv[h].y, acc[i][2 * h + 1]);
+                                }
                             }
                         }
                     }
@@ -604,10 +611,11 @@ cudaError_t launch_prompt_plan(const PromptLaunch& L, cudaStream_t stream) {
 cudaError_t launch_prompt_rows(const PromptLaunch& L, cudaStream_t stream) {
     const PromptArgs a = prompt_args(L);
     const bool bf = L.g.dtype == PP_DTYPE_BF16;
-    // resident CTAs an SM by shared memory: 3 at head_dim 64, 1 at 128
+    // As many CTAs as are resident at a time, by registers 2 an SM at head_dim 64 and by shared memory 1 at 128:
+    // one that waits for its turn would sit on its first unit until another CTA ends.
     if (L.g.head_dim == 64)
-        return bf ? launch_rows<64, true>(a, 3 * L.layout.max_ctas, stream)
-                  : launch_rows<64, false>(a, 3 * L.layout.max_ctas, stream);
+        return bf ? launch_rows<64, true>(a, 2 * L.layout.max_ctas, stream)
+                  : launch_rows<64, false>(a, 2 * L.layout.max_ctas, stream);
     return bf ? launch_rows<128, true>(a, L.layout.max_ctas, stream) : launch_rows<128, false>(a, L.layout.max_ctas, stream);
 }
 
