@@ -16,7 +16,10 @@ SyntheticDecoder runs the batched decode step of PrimitiveModel
 QKV projection -> q/k RMSNorm + RoPE + int8 append -> int8 decode attention
 (history + the current token as f32 scratch) -> output projection + residual
 -> RMSNorm -> gate/up projection -> SwiGLU -> down projection + residual, then
-the final RMSNorm.  The projections are cuBLAS GEMMs (torch.matmul), as the
+the final RMSNorm.  SyntheticDecoder.prefill takes whole prompts through the
+same layers at once (forward_embedding's query_length > 1 path, mod.rs:621-747):
+the prompt's tokens attend to each other in bf16 or f32, and their K/V are
+appended to the arenas.  The projections are cuBLAS GEMMs (torch.matmul), as the
 reference's are (`x.matmul(&w.t())`, batch.rs:134,155-170); everything else
 is this library's kernels.
 """
@@ -30,6 +33,7 @@ import numpy as np
 import torch
 
 from . import _native as N
+from . import fused_attention
 from . import int8_kv_ops as ops
 from . import kv_cache
 
@@ -284,6 +288,51 @@ class SyntheticDecoder:
             swiglu(gate_up, out=b["act"])
             residual = self._linear(b["act"], li, "down")
         return rmsnorm(xr, self.final_norm, residual=residual, x_sum=xr, out=b["out"])
+
+
+    def prefill(self, x: torch.Tensor, lengths: list[int], *, probe=None) -> torch.Tensor:
+        """Takes the first lengths[b] tokens of every branch through the model.
+
+        x [sum(lengths), width]: the input embeddings, branch after branch (it
+        is consumed, as step's).  Causal attention runs over the tokens' own
+        K/V; their int8 codes fill slots 0 .. lengths[b] of each arena, ready
+        for step(past=lengths).  A length may be 0: that branch's slots stay as
+        they are.  Returns the final-normed hidden state of every token
+        [sum(lengths), width].  probe(layer, q, k, v, arena, attention_out)
+        is called after each layer's attention is enqueued."""
+        cfg = self.cfg
+        H, d, tokens = cfg.heads, cfg.head_dim, sum(lengths)
+        if len(lengths) != self.branches or min(lengths) < 0 or max(lengths) > min(self.capacity, cfg.max_context):
+            raise N.PreconditionError("prefill needs one length a branch, within the arena and the RoPE table")
+        if tuple(x.shape) != (tokens, cfg.width) or x.dtype != self.dtype or x.device != self.device \
+                or not x.is_contiguous():
+            raise N.PreconditionError("prefill needs dense embeddings [sum(lengths), width] of the model's type")
+        if tokens == 0:
+            return torch.empty_like(x)
+        at = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+        starts = torch.from_numpy(at).to(self.device)
+        positions = torch.from_numpy(np.concatenate([np.arange(n, dtype=np.int32) for n in lengths])).to(self.device)
+        offsets = torch.zeros(self.branches, dtype=torch.int32, device=self.device)
+        normed = torch.empty_like(x)
+        planes = torch.empty((3, tokens, H, d), dtype=self.dtype, device=self.device)
+        q, k, v = planes.unbind(0)
+        att = torch.empty_like(q)
+        # one plan for every layer's attention
+        workspace = fused_attention.prompt_workspace(q, k, v, self.branches)
+        fused_attention.plan_prompt(q, k, v, starts, workspace, status=self.status)
+        residual = None
+        for li, (L, arena) in enumerate(zip(self.layers, self.arenas)):
+            rmsnorm(x, L["norm1"], residual=residual, x_sum=x if residual is not None else None, out=normed)
+            qkv_rope(self._linear(normed, li, "qkv"), L["rope"], positions, H, d, cfg.max_context,
+                     out=planes.view(3, tokens * H, d), status=self.status)
+            arena.append_prompt(k, v, starts, offsets, status=self.status)
+            fused_attention.prompt_attention(q, k, v, starts, workspace=workspace, plan_ready=True, out=att,
+                                             status=self.status)
+            if probe is not None:
+                probe(li, q, k, v, arena, att)
+            rmsnorm(x, L["norm2"], residual=self._linear(att.view(tokens, H * d), li, "proj"), x_sum=x, out=normed)
+            residual = self._linear(swiglu(self._linear(normed, li, "gate_up")), li, "down")
+        return rmsnorm(x, self.final_norm, residual=residual, x_sum=x)
 
 
 class CapturedStep:
