@@ -157,8 +157,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    pdl_launch_dependents();  // the merge may be set up meanwhile; it waits for this kernel before it reads
     pdl_wait_primary();
+    pdl_launch_dependents();  // after the wait: what a dependent reads early, kernels before this one have finished writing
 
     auto give_up = [&] {
         *abort = 1;

@@ -30,9 +30,7 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
                  : "memory");
 }
 
-// mbar_wait_bounded with the limit in SM clock cycles: %globaltimer takes about
-// a microsecond to read, which a wait that is over after a few hundred cycles
-// would feel at every key tile.
+// mbar_wait_bounded with the limit in SM clock cycles.
 __device__ __forceinline__ bool mbar_wait_cycles(uint64_t* bar, uint32_t parity, volatile int* abort, long long limit) {
     if (mbar_try_wait(bar, parity)) return true;
     const long long start = clock64();
@@ -45,35 +43,6 @@ __device__ __forceinline__ bool mbar_wait_cycles(uint64_t* bar, uint32_t parity,
 // bf16 operands, f32 accumulator: A [M, K] K-major, B [N, K] K-major or (mn) [K, N].
 __host__ __device__ constexpr uint32_t tc_bf16_desc(uint32_t m, uint32_t n, bool b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
-}
-
-// The matrix instructions and the commit below are for a whole warp, with uniform
-// arguments: one lane of it issues, always the same.
-
-// D[tmem] (+)= A[smem] B[smem].
-__device__ __forceinline__ void tc_mma_ss_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-        : "memory");
-}
-
-// D[tmem] (+)= A[tmem] B[smem].
-__device__ __forceinline__ void tc_mma_ts_elect(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-        : "memory");
-}
-
-// Arrives on `bar` when every matrix instruction that the lane issued so far is complete.
-__device__ __forceinline__ void tc_commit_elect(uint64_t* bar) {
-    asm volatile(
-        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar))
-        : "memory");
 }
 
 // D[tmem] (+)= A[smem] B[smem]; one thread issues.
