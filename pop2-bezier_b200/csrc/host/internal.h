@@ -135,15 +135,14 @@ struct AttnLaunch {
 //   cuts      u32 [max_ctas]                first piece of each cut entry
 //   acc       f32 [slots][slot_rows][head_dim]   partials of cut items
 //   ml        f32 [slots][slot_rows][2]          their maximum (log2 units), sum
-// An entry is cut only when its keys are more than its share of all the work,
-// (work in key tiles) / max_ctas, into ceil(keys / share) <= 2 keys / share
-// pieces: at most 2 max_ctas slots and max_ctas cut items, kv_heads included.
+// An entry is cut only when its steps (prompt.cu) are more than `limit`, one and a
+// half times the share (all steps) / max_ctas, into ceil(steps / limit) <= 2 steps /
+// limit pieces: at most 2 max_ctas slots and max_ctas cut items, kv_heads included.
 struct PromptHeader {
-    uint32_t n_entries;
     uint32_t n_items;  // entries * kv_heads
     uint32_t next;     // next item to hand out beyond the grid's first ones (zero between calls)
     uint32_t n_cuts;   // entries cut along their keys
-    uint32_t pad[4];
+    uint32_t pad[5];
 };
 
 struct PromptEntry {

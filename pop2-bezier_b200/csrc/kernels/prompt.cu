@@ -14,15 +14,19 @@ namespace {
 // key tiles where only one has rows), and writes them longest first (64 classes
 // of length), because the attention CTAs take items in this order as they
 // become free: the last ones taken are the shortest.  Where the whole batch has
-// fewer steps than it takes to keep every CTA busy with whole entries, an entry
-// of more than one and a half times its share, and of at least kCutSteps, is cut
-// into equal pieces along the keys; below that, the partials, the merge and the
-// uneven last round cost what the cut gains (the merge launch and the partials take
-// about as long as four steps).
+// fewer steps than it takes to keep every CTA busy with whole entries, entries of
+// more than one and a half times their share are cut into equal pieces along the
+// keys.  Pieces nearer to the share leave less room for the uneven last round (2048
+// causal tokens of 16 heads of 128: 43 us at 1.5, 51 at 1; 512 tokens at the end of
+// 32768, 16 heads on 2: 134 and 208); longer ones leave SMs without work (172 at 2).
+// Uncut it takes 450 us, and one sequence of 8192, one head of 64, 109 against 38.
+// Nothing is cut where no entry has kCutSteps: partials and their merge take about
+// as long as three steps (768 tokens, 8 heads of 64, cut from 6 steps on: 20.5 us
+// against 19.8; 2000 keys of one token, cut: 21 against 30).
 constexpr int kPlanThreads = 1024;
 constexpr uint32_t kClasses = 64;
 constexpr uint32_t kBaseMax = 2048;  // sequences whose first entries are kept in shared memory
-constexpr uint32_t kCutSteps = 12;
+constexpr uint32_t kCutSteps = 8;
 
 struct PlanArgs {
     const uint32_t* q_starts;
@@ -146,15 +150,19 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
     unsigned long long all = warp_work[lane];
 #pragma unroll
     for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-    all *= a.kv_heads;
-    const unsigned long long share = (all + a.l.max_ctas - 1) / a.l.max_ctas;
-    const uint32_t limit = (uint32_t)max(2ull, min(share + share / 2, 0x7fffffffull));
+    const float share = __fdividef((float)all * a.kv_heads, a.l.max_ctas);  // to a few units of 2^-24, which is plenty
     const uint32_t most = longest;
-    // pieces of an entry and the class of their length (steps < 2^25, so the product fits)
+    const uint32_t limit = most < kCutSteps ? most : (uint32_t)fminf(fmaxf(2.f, ceilf(1.5f * share)), 1e9f);
+    const float per_step = __fdividef((float)kClasses, most);
+    // pieces of an entry and the class of their length
     auto cut = [&](const Whole& w, uint32_t& pieces) {
-        pieces = w.steps < kCutSteps ? 1u : (w.steps + limit - 1) / limit;
-        const uint32_t len = (w.steps + pieces - 1) / pieces;
-        return kClasses - 1 - (len - 1) * kClasses / most;
+        pieces = 1;
+        uint32_t len = w.steps;
+        if (len > limit) {
+            pieces = (len + limit - 1) / limit;
+            len = (len + pieces - 1) / pieces;
+        }
+        return kClasses - 1 - min(kClasses - 1, (uint32_t)((len - 1) * per_step));
     };
     for (uint32_t e = t; e < n; e += kPlanThreads) {
         uint32_t pieces;
@@ -172,7 +180,6 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
         cursor[2 * t] = inc - lo - hi;
         cursor[2 * t + 1] = inc - hi;
         if (t == 31) {
-            hdr->n_entries = inc;
             hdr->n_items = inc * a.kv_heads;
             hdr->next = 0;
         }
@@ -465,16 +472,21 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) prompt_rows_ker
 
 // --------------------------------------------------- the pieces of cut rows
 //
-// A warp merges a row: out = sum_s 2^(m_s - m) acc_s / sum_s 2^(m_s - m) z_s over
-// its pieces in their order, whoever finished last.  Merging inside the attention
+// A warp merges four rows side by side: out = sum_s 2^(m_s - m) acc_s / sum_s 2^(m_s - m) z_s over
+// its pieces, a lane in 8 taking every eighth piece's m and z, in an order that
+// does not depend on who finished first.  It is a chain of dependent loads (header,
+// cut, entry, maxima, partials), so rows run side by side: 8 MB of partials, from
+// L2, take about 4 us, one row at a time took 10.  Merging inside the attention
 // kernels, by the CTA that brings an entry's last piece, took 17 to 33 thousand
-// cycles (one CTA's loads, and code that only it runs); spread over the GPU this
-// takes two or three microseconds, and one where nothing is cut.
-constexpr int kMergeWarps = 8;
+// cycles.
+constexpr uint32_t kMergeWarps = 8, kMergeRows = 4;  // rows of a warp at a time
 
 template <int D, bool BF>
 __global__ void __launch_bounds__(32 * kMergeWarps) prompt_merge_kernel(const __grid_constant__ PromptArgs a) {
     constexpr int C = D / 32;  // channels of a lane
+    struct alignas(4 * C) Lane {
+        float f[C];
+    };
     const uint32_t lane = threadIdx.x & 31;
     const PromptHeader* hdr = reinterpret_cast<const PromptHeader*>(a.ws);
     const PromptEntry* entries = reinterpret_cast<const PromptEntry*>(a.ws + a.l.entries);
@@ -482,54 +494,72 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prompt_merge_kernel(const __
     const float* acc = reinterpret_cast<const float*>(a.ws + a.l.acc);
     const float* ml = reinterpret_cast<const float*>(a.ws + a.l.ml);
     pdl_wait_primary();
-    const uint32_t groups = hdr->n_cuts * a.kv_heads, rows = a.l.slot_rows;
-    for (uint64_t i = (uint64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5); i < (uint64_t)groups * rows;
-         i += (uint64_t)gridDim.x * kMergeWarps) {
-        const uint32_t row = (uint32_t)(i % rows), head = (uint32_t)(i / rows) % a.kv_heads;
-        const PromptEntry e = entries[cuts[(uint32_t)(i / rows) / a.kv_heads]];
-        const uint32_t r = row % kPromptTileRows;  // of its tile
-        const uint32_t token = e.tok0 + row / kPromptTileRows * a.tpt + r / a.group;
-        if (r >= a.tpt * a.group || token >= e.nq) continue;
-        const uint64_t first = ((uint64_t)e.slot0 * a.kv_heads + head) * rows + row, step = (uint64_t)a.kv_heads * rows;
-        float m = -CUDART_INF_F, z = 0.f, o[C];
-        for (uint32_t s = lane; s < e.n_splits; s += 32) m = fmaxf(m, ml[2 * (first + s * step)]);
+    const uint32_t groups = hdr->n_cuts * a.kv_heads, rows = a.l.slot_rows, quads = rows / kMergeRows;
+    const uint32_t sub = lane / 8, piece = lane % 8;
+    for (uint32_t i = blockIdx.x * kMergeWarps + (threadIdx.x >> 5); i < groups * quads; i += gridDim.x * kMergeWarps) {
+        const uint32_t row0 = i % quads * kMergeRows, head = i / quads % a.kv_heads;
+        const PromptEntry e = entries[cuts[i / quads / a.kv_heads]];
+        auto token_of = [&](uint32_t row) {
+            return e.tok0 + row / kPromptTileRows * a.tpt + row % kPromptTileRows / a.group;
+        };
+        auto exists = [&](uint32_t row) { return row % kPromptTileRows < a.tpt * a.group && token_of(row) < e.nq; };
+        const uint64_t first = ((uint64_t)e.slot0 * a.kv_heads + head) * rows + row0, step = (uint64_t)a.kv_heads * rows;
+        const float2* mz = reinterpret_cast<const float2*>(ml) + first + sub;  // of the lane's row
+        const bool mine = exists(row0 + sub);
+        const uint32_t live = __ballot_sync(0xffffffffu, mine);
+        float m = -CUDART_INF_F, z = 0.f;
+        Lane o[kMergeRows] = {};
+        for (uint32_t s = piece; s < e.n_splits; s += 8)
+            if (mine) m = fmaxf(m, mz[s * step].x);
 #pragma unroll
-        for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+        for (int k = 4; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
         const float ref = m == -CUDART_INF_F ? 0.f : m;
-#pragma unroll
-        for (int c = 0; c < C; ++c) o[c] = 0.f;
-        for (uint32_t s0 = 0; s0 < e.n_splits; s0 += 32) {
-            float w = 0.f, zs = 0.f;
-            if (s0 + lane < e.n_splits) {
-                const float2 mz = *reinterpret_cast<const float2*>(ml + 2 * (first + (s0 + lane) * step));
-                if (mz.y != 0.f) w = exp2f(mz.x - ref);  // 0: the row saw nothing of this piece
-                zs = mz.y * w;
+        for (uint32_t s0 = 0; s0 < e.n_splits; s0 += 8) {
+            float w = 0.f;
+            if (mine && s0 + piece < e.n_splits) {
+                const float2 p = mz[(s0 + piece) * step];
+                if (p.y != 0.f) w = exp2f(p.x - ref);  // 0: the row saw nothing of this piece
+                z += p.y * w;
             }
-            const uint32_t n = min(32u, e.n_splits - s0);
-#pragma unroll 4
+            const uint32_t n = min(8u, e.n_splits - s0);
+#pragma unroll 2
             for (uint32_t s = 0; s < n; ++s) {
-                float x[C];
+                Lane x[kMergeRows];
 #pragma unroll
-                for (int c = 0; c < C; ++c) x[c] = acc[(first + (s0 + s) * step) * D + C * lane + c];
-                const float ws = __shfl_sync(0xffffffffu, w, s);
-                z += __shfl_sync(0xffffffffu, zs, s);
+                for (uint32_t u = 0; u < kMergeRows; ++u)
+                    if (live >> 8 * u & 1u)
+                        x[u] = *reinterpret_cast<const Lane*>(acc + (first + (s0 + s) * step + u) * D + C * lane);
 #pragma unroll
-                for (int c = 0; c < C; ++c)
-                    if (ws != 0.f) o[c] += x[c] * ws;
+                for (uint32_t u = 0; u < kMergeRows; ++u) {
+                    const float ws = __shfl_sync(0xffffffffu, w, 8 * u + s);
+                    if (ws == 0.f) continue;
+#pragma unroll
+                    for (int c = 0; c < C; ++c) o[u].f[c] += x[u].f[c] * ws;
+                }
             }
         }
-        const uint64_t at = ((uint64_t)(e.q0 + token) * a.heads + head * a.group + r % a.group) * D + C * lane;
-        const float inv = z == 0.f ? CUDART_NAN_F : 1.f / z;  // a row that sees no key
-        bool bad = false;
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            o[c] *= inv;
-            bad = bad || !(o[c] * 0.f == 0.f);
-            if constexpr (BF) reinterpret_cast<__nv_bfloat16*>(a.out)[at + c] = __float2bfloat16_rn(o[c]);
-            else reinterpret_cast<float*>(a.out)[at + c] = o[c];
-        }
-        if constexpr (BF) {
-            if (a.vec && __any_sync(0xffffffffu, bad) && z != 0.f) redo_row<D>(a, e, head, token, r % a.group);
+        for (int k = 4; k; k >>= 1) z += __shfl_xor_sync(0xffffffffu, z, k);
+#pragma unroll
+        for (uint32_t u = 0; u < kMergeRows; ++u) {
+            if (!(live >> 8 * u & 1u)) continue;
+            const uint32_t token = token_of(row0 + u), g = (row0 + u) % kPromptTileRows % a.group;
+            const float zu = __shfl_sync(0xffffffffu, z, 8 * u), inv = zu == 0.f ? CUDART_NAN_F : 1.f / zu;  // no key seen
+            const uint64_t at = ((uint64_t)(e.q0 + token) * a.heads + head * a.group + g) * D + C * lane;
+            float chk = 0.f;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                o[u].f[c] *= inv;
+                chk = fmaf(o[u].f[c], 0.f, chk);
+            }
+            if constexpr (BF) {
+#pragma unroll
+                for (int c = 0; c < C; c += 2)
+                    reinterpret_cast<uint32_t*>(a.out)[(at + c) / 2] = pack_bf16x2(o[u].f[c], o[u].f[c + 1]);
+                if (a.vec && zu != 0.f && __any_sync(0xffffffffu, !(chk == 0.f))) redo_row<D>(a, e, head, token, g);
+            } else {
+                *reinterpret_cast<Lane*>(reinterpret_cast<float*>(a.out) + at) = o[u];
+            }
         }
     }
 }
@@ -624,7 +654,7 @@ uint32_t prompt_uncut_keys() { return (kCutSteps - 1) * kPromptKeyTile; }
 
 cudaError_t launch_prompt_merge(const PromptLaunch& L, cudaStream_t stream) {
     const PromptArgs a = prompt_args(L);
-    const dim3 grid(2 * L.num_sms), block(32 * kMergeWarps);
+    const dim3 grid(4 * L.num_sms), block(32 * kMergeWarps);
     const bool bf = L.g.dtype == PP_DTYPE_BF16;
     if (L.g.head_dim == 64)
         return bf ? launch_pdl(prompt_merge_kernel<64, true>, grid, block, stream, a)

@@ -237,6 +237,35 @@ def test_cut_and_whole_plans_agree_and_repeat_bit_for_bit(pp, cuda, dtype, max_c
     check(o2, q2, k2, v2, q_lens, kv_lens, True)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("past", [900, 1500, 20000])
+def test_rows_cut_into_pieces(pp, cuda, past, d, dtype):
+    """Few rows over many keys: two to more than eight pieces, tiles with rows that do not exist, a value that is
+    not finite and that only the last tokens see."""
+    q_lens = [50, 1, 90, 7]
+    kv_lens = [50 + past, 1 + past // 2, 90 + past // 3, 7]
+    q, k, v = tensors(cuda, sum(q_lens), sum(kv_lens), 6, 2, d, dtype, seed=past)
+    v[sum(kv_lens[:1]) - 2] = math.nan
+    v[sum(kv_lens[:3]) - 1, 0] = math.inf
+    v[sum(kv_lens[:3]) - 1, 0, 3] = math.nan
+    out = pp.fused_attention.prompt_attention(q, k, v, starts_of(q_lens, cuda), kv_starts=starts_of(kv_lens, cuda))
+    at_q, at_k = 0, 0
+    for n, m in zip(q_lens, kv_lens):
+        rows, keys = slice(at_q, at_q + n), slice(at_k, at_k + m)
+        want, err = exact_rows(q[rows], k[keys], v[keys].masked_fill(v[keys].isinf(), 0.0), True, d**-0.5)
+        # the channels of K/V head 0 that the last token sees as inf
+        inf = torch.zeros(n, 2, d, dtype=torch.bool, device=cuda)
+        inf[n - 1] = v[keys][m - 1].isinf()
+        inf = inf.repeat_interleave(3, 1)
+        got = out[rows].double()
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.isinf(), inf & ~want.isnan())
+        plain = ~inf & ~want.isnan()
+        assert not (((got - want).abs() > err) & plain).any()
+        at_q, at_k = at_q + n, at_k + m
+
+
 @pytest.mark.parametrize("sequences", [1500, 40])
 def test_many_short_sequences(pp, cuda, sequences):
     """More sequences than the plan's threads, most of them shorter than a tile."""
