@@ -275,13 +275,15 @@ size_t pp_b200_prompt_workspace_size(const PpPrompt* prompt);
 /* The work list of these sequences: tiles of query rows, longest first, and
  * cut along the keys where there are too few of them to fill the GPU.  Every
  * layer of a step reuses it with PP_ATTN_PLAN_READY (same geometry, strides
- * apart, and same lengths).  q, k and v may be NULL here.
+ * apart, same max_ctas and same lengths).  q, k and v may be NULL here.  The
+ * workspace belongs to one call at a time.
  * status (nullable): PP_DEV_LENGTH_RANGE. */
 int32_t pp_b200_plan_prompt(const PpPrompt* prompt, const uint32_t* q_starts, const uint32_t* kv_starts,
                             void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
 
 /* Attention of every query token over its own sequence, scores, softmax and
- * sums in f32.  out: [q_tokens, heads, head_dim] of the prompt's dtype, dense.
+ * sums in f32.  out: [q_tokens, heads, head_dim] of the prompt's dtype, dense,
+ * not overlapping q, k or v.
  * status (nullable): PP_DEV_LENGTH_RANGE, PP_DEV_WAIT_TIMEOUT. */
 int32_t pp_b200_prompt_attention(const PpPrompt* prompt, const uint32_t* q_starts, const uint32_t* kv_starts,
                                  void* out, void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
@@ -315,7 +317,7 @@ int32_t pp_b200_prompt_append(const PpKvArena* arena, const void* k, const void*
  *   top_ids, top_logprobs  u32 / f32 [rows, top], the first `top` (0 .. 32) of
  *             that order; 0xffffffff and -inf beyond the window and for
  *             columns whose logit is -inf.  NULL with top 0.
- * Sums are in f32, the closing logarithm in f64.  A NaN or +inf logit in the
+ * Sums and logarithm are in f32.  A NaN or +inf logit in the
  * window makes the row's logprob, entropy and top_logprobs NaN, as log-softmax
  * does; NaN logits come last in the order (after -inf, and in no list of
  * alternatives).  An empty window gives NaN, no alternatives and rank 0; one

@@ -186,7 +186,7 @@ int32_t pp_b200_token_logprobs(const void* logits, int32_t dtype, uint32_t rows,
                                float* top_logprobs, uint32_t* status, void* stream) {
     if (dtype != PP_DTYPE_F32 && dtype != PP_DTYPE_BF16)
         return fail_fmt(PP_STATUS_PRECONDITION, "token logprobs: unsupported dtype %d", dtype);
-    if (choices == 0 || choices > 0x7fffffffu || rows > 0x7fffffffu || top > 32)
+    if (choices == 0 || choices > 0x7fffff00u || rows > 0x7fffffffu || top > 32)
         return fail_fmt(PP_STATUS_PRECONDITION,
                         "token logprobs need a nonempty head and at most 32 alternatives: rows=%u choices=%u top=%u", rows,
                         choices, top);

@@ -37,9 +37,9 @@
 namespace pp {
 namespace {
 
-constexpr int kVecs = 8;              // 16-byte vectors a lane holds
+constexpr int kVecs = 8;              // 16-byte vectors of a thread in a step
 constexpr uint32_t kCandidates = 64;  // of a warp
-constexpr int kMostWarps = 8;          // of a CTA
+constexpr uint32_t kMostWarps = 8;    // of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
             p.ahead += __shfl_xor_sync(0xffffffffu, p.ahead, o);
         }
     }
-    if (NW == kMostWarps && a.cluster > 1) {
+    if (NW == (int)kMostWarps && a.cluster > 1) {
         if (threadIdx.x == 0) s_cta = p;
         if (warp == 0 && current) s_list[0][lane] = s_list[1][lane];  // peers look at the first
         cluster_sync();
@@ -632,13 +632,12 @@ cudaError_t launch_token_logprobs(const LogprobsLaunch& L, cudaStream_t stream) 
     a.top_logprobs = L.top_logprobs;
     a.status = L.status;
     a.cluster = 1;
-    // As many warps as the row has 4 KB, up to 16; with too few rows to give
-    // every SM one, 8 warps and a cluster of CTAs for what is longer.
+    // As many warps as the row has 4 KB, up to 8; with too few rows to give every SM
+    // one, 8 warps and a cluster of CTAs for what is longer.
     const uint64_t parts = ((uint64_t)L.choices * (L.bf16 ? 2 : 4) + 4095) / 4096;
-    const uint32_t most = kMostWarps;
     uint32_t warps = 1;
-    while (warps < most && warps < parts) warps *= 2;
-    while (a.cluster < 8 && (uint64_t)L.rows * a.cluster * 2 <= 2ull * L.num_sms && (uint64_t)warps * a.cluster < parts)
+    while (warps < kMostWarps && warps < parts) warps *= 2;
+    while (a.cluster < 8 && (uint64_t)L.rows * a.cluster <= L.num_sms && (uint64_t)warps * a.cluster < parts)
         a.cluster *= 2;
     return L.bf16 ? launch_warps<true>(a, warps, stream) : launch_warps<false>(a, warps, stream);
 }

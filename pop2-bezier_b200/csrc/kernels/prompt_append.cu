@@ -27,7 +27,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxChunk = 64;  // tokens of a CTA
 constexpr int kE = 16;         // elements of a lane
-constexpr int kRows = 1;       // rows that a lane has in flight; two cost more registers than they hide latency
 
 struct AppendArgs {
     const void* src[2];  // K, V
@@ -195,67 +194,59 @@ __global__ void __launch_bounds__(kThreads) prompt_append_kernel(const AppendArg
     uint32_t tok = threadIdx.x / L / a.heads, head = threadIdx.x / L % a.heads;
     uint64_t next_from = (uint64_t)(t0 + tok) * ts + head * hs + kE * lane, next_row = (uint64_t)head * a.capacity;
     bool finite = true;
-    for (uint32_t r0 = 0; r0 < rows; r0 += kRows * R) {  // the same number of turns for all of the block
-        Raw<BF> raw[kRows];
-        uint64_t slot[kRows], from[kRows];
-#pragma unroll
-        for (int u = 0; u < kRows; ++u) {
-            slot[u] = tok < n_tok ? dst[tok] : ~0ull;
-            from[u] = next_from;
-            raw[u] = Raw<BF>{};
-            if (slot[u] != ~0ull) {
-                slot[u] += next_row;
-                raw[u] = load_raw<BF>(src, next_from, a.vec);
-            }
-            tok += step_tok;
-            head += step_head;
-            next_from += step_from;
-            next_row += step_row;
-            if (head >= a.heads) {
-                head -= a.heads;
-                ++tok;
-                next_from += wrap_from;
-                next_row -= wrap_row;
-            }
+    for (uint32_t r0 = 0; r0 < rows; r0 += R) {  // the same number of turns for all of the block
+        uint64_t slot = tok < n_tok ? dst[tok] : ~0ull;
+        const uint64_t from = next_from;
+        Raw<BF> raw{};
+        if (slot != ~0ull) {
+            slot += next_row;
+            raw = load_raw<BF>(src, from, a.vec);
         }
+        tok += step_tok;
+        head += step_head;
+        next_from += step_from;
+        next_row += step_row;
+        if (head >= a.heads) {
+            head -= a.heads;
+            ++tok;
+            next_from += wrap_from;
+            next_row -= wrap_row;
+        }
+        float v[kE], m = largest<BF>(raw);
+        unpack<BF>(raw, v);
 #pragma unroll
-        for (int u = 0; u < kRows; ++u) {
-            float v[kE], m = largest<BF>(raw[u]);
-            unpack<BF>(raw[u], v);
+        for (int o = L / 2; o; o >>= 1) {
+            const float y = __shfl_xor_sync(0xffffffffu, m, o);
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(y));
+        }
+        float s = fmaxf(over_127(m), 1e-12f);
+        const float y = __frcp_rn(s);
+        const uint64_t y2 = f2_pack(y, y), s2 = f2_pack(-s, -s), up = f2_pack(12582912.f, 12582912.f);
+        uint32_t w[kE / 4];
 #pragma unroll
-            for (int o = L / 2; o; o >>= 1) {
-                const float y = __shfl_xor_sync(0xffffffffu, m, o);
-                asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(y));
-            }
-            float s = fmaxf(over_127(m), 1e-12f);
-            const float y = __frcp_rn(s);
-            const uint64_t y2 = f2_pack(y, y), s2 = f2_pack(-s, -s), up = f2_pack(12582912.f, 12582912.f);
-            uint32_t w[kE / 4];
+        for (int k = 0; k < kE; k += 4) {
+            float c[4];
 #pragma unroll
-            for (int k = 0; k < kE; k += 4) {
-                float c[4];
-#pragma unroll
-                for (int h = 0; h < 4; h += 2) {
-                    const uint64_t x = f2_pack(v[k + h], v[k + h + 1]);
-                    uint64_t q = f2_mul(x, y2);
-                    q = f2_fma(f2_fma(q, s2, x), y2, q);
-                    q = f2_fma(f2_fma(q, s2, x), y2, q);
-                    f2_unpack(f2_add(q, up), c[h], c[h + 1]);
-                }
-                w[k / 4] = __byte_perm(__byte_perm(__float_as_uint(c[0]), __float_as_uint(c[1]), 0x0040),
-                                       __byte_perm(__float_as_uint(c[2]), __float_as_uint(c[3]), 0x0040), 0x5410);
+            for (int h = 0; h < 4; h += 2) {
+                const uint64_t x = f2_pack(v[k + h], v[k + h + 1]);
+                uint64_t q = f2_mul(x, y2);
+                q = f2_fma(f2_fma(q, s2, x), y2, q);
+                q = f2_fma(f2_fma(q, s2, x), y2, q);
+                f2_unpack(f2_add(q, up), c[h], c[h + 1]);
             }
-            uint4 codes = make_uint4(w[0], w[1], w[2], w[3]);
-            if (!isfinite(m)) {  // all the row's lanes
-                const Divided d = divided<D, BF>(src, from[u], a.vec);
-                codes = d.codes;
-                s = d.s;
-                finite = finite && d.finite;
-            }
-            if (slot[u] != ~0ull) {
-                *reinterpret_cast<uint4*>(arena + slot[u] * D + kE * lane) = codes;
-                if (lane == 0) scales[slot[u]] = s;
-            }
+            w[k / 4] = __byte_perm(__byte_perm(__float_as_uint(c[0]), __float_as_uint(c[1]), 0x0040),
+                                   __byte_perm(__float_as_uint(c[2]), __float_as_uint(c[3]), 0x0040), 0x5410);
+        }
+        uint4 codes = make_uint4(w[0], w[1], w[2], w[3]);
+        if (!isfinite(m)) {  // all the row's lanes
+            const Divided d = divided<D, BF>(src, from, a.vec);
+            codes = d.codes;
+            s = d.s;
+            finite = finite && d.finite;
+        }
+        if (slot != ~0ull) {
+            *reinterpret_cast<uint4*>(arena + slot * D + kE * lane) = codes;
+            if (lane == 0) scales[slot] = s;
         }
     }
     if (!finite && a.status) atomicOr(a.status, PP_DEV_NONFINITE_INPUT);
@@ -284,7 +275,7 @@ cudaError_t launch_prompt_append(const PromptAppendLaunch& P, cudaStream_t strea
     a.vec = P.vec;
     a.status = P.status;
     // About 24 CTAs an SM where the prompts are long, at least one turn of rows each where they are short.
-    const uint32_t turn = kRows * kThreads / (P.arena->head_dim / kE);
+    const uint32_t turn = kThreads / (P.arena->head_dim / kE);
     uint32_t chunk = P.tokens / (12 * P.num_sms);
     chunk = chunk > (turn + a.heads - 1) / a.heads ? chunk : (turn + a.heads - 1) / a.heads;
     a.chunk = chunk < kMaxChunk ? chunk : kMaxChunk;

@@ -95,7 +95,7 @@ def test_append_arena(pp):
         assert N.lib.pp_b200_prompt_append(*args) == N.STATUS_PRECONDITION, field
 
 
-@pytest.mark.parametrize("bad", [dict(dtype=5), dict(choices=0), dict(choices=2**31), dict(rows=2**31), dict(top=33),
+@pytest.mark.parametrize("bad", [dict(dtype=5), dict(choices=0), dict(choices=2**31), dict(choices=2**31 - 1), dict(rows=2**31), dict(top=33),
                                  dict(stride=2**40)], ids=str)
 def test_logprobs(pp, bad):
     N = pp._native
