@@ -23,7 +23,7 @@ namespace {
 // Nothing is cut where no entry has kCutSteps: partials and their merge take about
 // as long as three steps (768 tokens, 8 heads of 64, cut from 6 steps on: 20.5 us
 // against 19.8; 2000 keys of one token, cut: 21 against 30).
-constexpr int kPlanThreads = 1024;
+constexpr uint32_t kPlanThreads = 1024;  // at most
 constexpr uint32_t kClasses = 64;
 constexpr uint32_t kBaseMax = 2048;  // sequences whose first entries are kept in shared memory
 constexpr uint32_t kCutSteps = 8;
@@ -93,13 +93,14 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
     __shared__ uint32_t warp_tot[32], hist[kClasses], cursor[kClasses], base_s[kBaseMax + 1];
     __shared__ unsigned long long warp_work[32];
     __shared__ uint32_t longest, slots, cuts;
-    const uint32_t t = threadIdx.x, lane = t & 31;
+    const uint32_t t = threadIdx.x, lane = t & 31, threads = blockDim.x;
     PromptHeader* hdr = reinterpret_cast<PromptHeader*>(a.ws);
     uint32_t* seq_base = a.sequences <= kBaseMax ? base_s : reinterpret_cast<uint32_t*>(a.ws + a.l.seq_base);
     PromptEntry* entries = reinterpret_cast<PromptEntry*>(a.ws + a.l.entries);
     uint32_t* cut_list = reinterpret_cast<uint32_t*>(a.ws + a.l.cuts);
     if (t == 0) longest = slots = cuts = 0;
-    if (t < kClasses) hist[t] = 0;
+    for (uint32_t c = t; c < kClasses; c += threads) hist[c] = 0;
+    if (t < 32) warp_work[t] = 0;
     // launched as a programmatic dependent: the kernels before may still read
     // the workspace or write the starts.  A dependent attention launch may
     // start now; it waits for this kernel before it reads the plan.
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
     pdl_launch_dependents();
     int bad = 0;
     uint32_t n = 0;
-    for (uint32_t b0 = 0; b0 < a.sequences; b0 += kPlanThreads) {
+    for (uint32_t b0 = 0; b0 < a.sequences; b0 += threads) {
         const uint32_t b = b0 + t;
         uint32_t nq = 0;
         if (b < a.sequences) {
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
     {
         unsigned long long mine = 0;
         uint32_t far = 0;
-        for (uint32_t e = t; e < n; e += kPlanThreads) {
+        for (uint32_t e = t; e < n; e += threads) {
             const uint32_t steps = e == t ? first.steps : entry_of(a, seq_base, e).steps;
             mine += steps;
             far = max(far, steps);
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
         }
         return kClasses - 1 - min(kClasses - 1, (uint32_t)((len - 1) * per_step));
     };
-    for (uint32_t e = t; e < n; e += kPlanThreads) {
+    for (uint32_t e = t; e < n; e += threads) {
         uint32_t pieces;
         const uint32_t c = e == t ? cut(first, pieces) : cut(entry_of(a, seq_base, e), pieces);
         atomicAdd(&hist[c], pieces);
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
         }
     }
     __syncthreads();
-    for (uint32_t e = t; e < n; e += kPlanThreads) {
+    for (uint32_t e = t; e < n; e += threads) {
         Whole w = e == t ? first : entry_of(a, seq_base, e);
         uint32_t pieces;
         const uint32_t at = atomicAdd(&cursor[cut(w, pieces)], pieces);
@@ -635,7 +636,11 @@ cudaError_t launch_prompt_plan(const PromptLaunch& L, cudaStream_t stream) {
     a.tpt = kPromptTileRows / (L.g.heads / L.g.kv_heads);
     a.kv_heads = L.g.kv_heads;
     a.status = L.status;
-    return launch_pdl(prompt_plan_kernel, dim3(1), dim3(kPlanThreads), stream, a);
+    // A thread an entry, if that many fit.
+    uint32_t threads = 32;
+    const uint64_t most = (uint64_t)L.g.q_tokens / (2 * a.tpt) + L.g.sequences;
+    while (threads < kPlanThreads && threads < most) threads *= 2;
+    return launch_pdl(prompt_plan_kernel, dim3(1), dim3(threads), stream, a);
 }
 
 cudaError_t launch_prompt_rows(const PromptLaunch& L, cudaStream_t stream) {
