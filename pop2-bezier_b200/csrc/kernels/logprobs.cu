@@ -175,12 +175,6 @@ __device__ __forceinline__ int rising(float x) {
 }
 __device__ __forceinline__ float rising_value(int k) { return __int_as_float(k ^ (k >> 31 & 0x7fffffff)); }
 
-__device__ __forceinline__ void copy16(uint4* to, const void* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(to)), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copies_sent() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
-
 // The list of the best 32 from the candidates and the list before it, by all of the block.
 __device__ __noinline__ void sort_candidates(const unsigned long long* cand, uint32_t count,
                                              const unsigned long long* old, unsigned long long* list, uint32_t k) {
@@ -237,8 +231,7 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
         const char* from = row_ptr + (int64_t)col0 * (BF ? 2 : 4);
         if (first + (int)v0 * EPV >= lo && v0 + STEP <= vectors && first + (int)(v0 + STEP) * EPV <= hi) {
 #pragma unroll
-            for (int v = 0; v < kVecs; ++v) copy16(to + v * T, from + v * T * 16);
-            copies_sent();
+            for (int v = 0; v < kVecs; ++v) cp_async16(to + v * T, from + v * T * 16);
             return;
         }
 #pragma unroll 1
@@ -246,7 +239,7 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
             const uint32_t at = v0 + v * T + threadIdx.x;
             const int col = col0 + v * T * EPV;
             if (at < vectors && col >= lo && col + EPV <= hi) {
-                copy16(to, from);
+                cp_async16(to, from);
                 continue;
             }
             const uint32_t none = BF ? 0xff80ff80u : 0xff800000u;  // -inf: an end of the window, or nothing
@@ -259,7 +252,6 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
                     else reinterpret_cast<uint32_t*>(to)[i] = bits;
                 }
         }
-        copies_sent();
     };
     const uint32_t stride = a.cluster * STEP;
     if (part * STEP < vectors) fetch(part * STEP);
@@ -279,7 +271,7 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
     bool over = false;  // candidates did not fit: the list is found in the row again
     __syncthreads();
     for (uint32_t v0 = part * STEP; v0 < vectors; v0 += stride, turn ^= 1) {
-        copies_landed();
+        cp_async_wait_all();
         float top = -CUDART_INF_F;
         if constexpr (BF) {
             uint32_t most = 0xff80ff80u;

@@ -249,7 +249,8 @@ __device__ __forceinline__ void store4(void* p, uint64_t i, float4 x) {
 template <int D>
 struct RowsCfg {
     static constexpr int LD = D + 4;  // rows 4 banks apart: 8 lanes' float4 cover all banks
-    static constexpr int SMEM = (2 * 64 * LD + 64 * D + 64 * (kBN + 4)) * 4;
+    static constexpr int KV = 64 * LD + 64 * D;  // a tile of keys and its values
+    static constexpr int SMEM = (64 * LD + 2 * KV + 64 * (kBN + 4)) * 4;
 };
 
 template <int D, bool BF>
@@ -258,9 +259,8 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) prompt_rows_ker
     constexpr int H = D / 64;  // channel groups of 4 a thread holds
     extern __shared__ __align__(16) float sm[];
     float* sq = sm;
-    float* sk = sq + 64 * C::LD;
-    float* sv = sk + 64 * C::LD;
-    float* sp = sv + 64 * D;
+    float* skv = sq + 64 * C::LD;
+    float* sp = skv + 2 * C::KV;
     __shared__ uint32_t s_next;
     const int t = threadIdx.x, tx = t & 15, ty = t >> 4;
     PromptHeader* hdr = reinterpret_cast<PromptHeader*>(a.ws);
@@ -307,20 +307,35 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) prompt_rows_ker
                 last = min(e.kv_end, prompt_visible(e, token_of(r_last), a.causal));
                 first = min(e.kv_end, prompt_visible(e, token_of(0), a.causal));
             }
-            for (uint32_t n0 = e.kv_begin; n0 < last; n0 += kBN) {
-                __syncthreads();
+            // The next tile is copied while this one is used (f32 on the 16-byte grid; other rows are converted on the way).
+            auto fetch = [&](uint32_t n0, float* sk) {
+                float* sv = sk + 64 * C::LD;
                 for (int i = t; i < 64 * (D / 4); i += kRowsThreads) {
                     const uint32_t r = i / (D / 4), c = i % (D / 4) * 4;
-                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+                    float *to_k = sk + r * C::LD + c, *to_v = sv + r * D + c;
                     if (n0 + r < last) {
                         const uint64_t row = (uint64_t)e.k0 + n0 + r;
-                        x = load4<BF>(a.k, row * a.k_ts + (uint64_t)head * a.k_hs + c, a.vec);
-                        y = load4<BF>(a.v, row * a.v_ts + (uint64_t)head * a.v_hs + c, a.vec);
+                        const uint64_t at_k = row * a.k_ts + (uint64_t)head * a.k_hs + c;
+                        const uint64_t at_v = row * a.v_ts + (uint64_t)head * a.v_hs + c;
+                        if (!BF && a.vec) {
+                            cp_async16(to_k, reinterpret_cast<const float*>(a.k) + at_k);
+                            cp_async16(to_v, reinterpret_cast<const float*>(a.v) + at_v);
+                            continue;
+                        }
+                        *reinterpret_cast<float4*>(to_k) = load4<BF>(a.k, at_k, a.vec);
+                        *reinterpret_cast<float4*>(to_v) = load4<BF>(a.v, at_v, a.vec);
+                    } else {
+                        *reinterpret_cast<float4*>(to_k) = *reinterpret_cast<float4*>(to_v) = make_float4(0.f, 0.f, 0.f, 0.f);
                     }
-                    *reinterpret_cast<float4*>(sk + r * C::LD + c) = x;
-                    *reinterpret_cast<float4*>(sv + r * D + c) = y;
                 }
-                __syncthreads();
+            };
+            uint32_t buf = 0;
+            if (e.kv_begin < last) fetch(e.kv_begin, skv);
+            for (uint32_t n0 = e.kv_begin; n0 < last; n0 += kBN, buf ^= 1) {
+                cp_async_wait_all();
+                __syncthreads();  // the tile is there, and nobody reads the other one any more
+                if (last - n0 > kBN) fetch(n0 + kBN, skv + (buf ^ 1) * C::KV);
+                const float *sk = skv + buf * C::KV, *sv = sk + 64 * C::LD;
                 uint64_t s2[4][4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
