@@ -13,22 +13,27 @@
 // A thread copies 8 vectors of 16 bytes into shared memory (cp.async) and looks at
 // them several times (maximum, sums, rank, alternatives) in short loops: nothing
 // waits for another thread's copies, and the loops stay in the instruction cache,
-// which the same code unrolled over registers did not (4096 rows of 32768: 154 us
-// against 95).  One buffer a CTA leaves room for five CTAs an SM, which hide the
+// which the same code unrolled over registers did not (4096 rows of 32768, with
+// the bound of that time: 154 us against 95).  One buffer a CTA leaves room for five CTAs an SM, which hide the
 // copies better than a second buffer with three (117 us).  NW warps take 4 KB each of a
 // row; a longer row is taken in steps, with one barrier each, or by a cluster of
 // up to 8 CTAs that merge through their shared memory, when there are few rows.
 //
-// Alternatives: with q = ceil(k / NW), the q-th largest lane maximum of ceil(k / q)
-// warps is reached by at least k logits, so the least of these is no larger than
-// the k-th best.  Only logits from the best such bound on are candidates (on
-// random rows a few times k of them); they wait in a buffer a warp until the row
-// ends or a buffer is half full.  A candidate's place in the list is the number
-// of candidates ahead of it, which one thread each counts.  Where a step leaves
-// more candidates than a buffer holds (long ties), the block takes the maximum k
-// times instead.
+// Alternatives: with q = ceil(k / NW), take every warp's q-th largest lane maximum;
+// the ceil(k / q)-th largest of these is reached by at least k logits, so it is no
+// larger than the k-th best.  Only logits from the best such bound on are candidates
+// (on random rows one or two times k of a step's); they wait in a buffer until the
+// row ends or a warp has used half its share of it.  A candidate's place in the list is the number of
+// candidates ahead of it, which one thread each counts; the order in which they were
+// found does not matter.  Where a step leaves more candidates than the buffer holds
+// (long ties), the block takes the maximum k times instead.
 //
-// Bound by HBM on long rows; issue slots and the latency of a step come next.
+// Bound by issue slots and the barrier of a step: 4096 rows of 32768 bf16 with 5
+// alternatives 81 us, 3.3 TB/s (maximum and sums alone 53, the rank 8, alternatives
+// 20); few rows by latency: 8 of 131072 with 20 alternatives 12 us; 2304 windows of
+// up to 1024 f32 9 us.  With the least of the first ceil(k / q) warps' values as the
+// bound there are twice the candidates: 100 us.  Candidates pushed lane by lane, with
+// an atomic each, instead of warp by warp: 98 us.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -129,12 +134,10 @@ __device__ __forceinline__ float picked(const uint4* p, int i) {
     else return reinterpret_cast<const float*>(p)[i];
 }
 
-// 1 in each half where a > b (ge: a >= b), as bf16; NaN gives 0.
-template <bool GE>
+// 1 in each half where a > b, as bf16; NaN gives 0.
 __device__ __forceinline__ uint32_t above_bf16x2(uint32_t a, uint32_t b) {
     uint32_t r;
-    if constexpr (GE) asm("set.ge.bf16x2.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    else asm("set.gt.bf16x2.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    asm("set.gt.bf16x2.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 __device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
@@ -318,11 +321,16 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
 #pragma unroll
         for (int w = 0; w < NW; ++w) m = fmaxf(m, rising_value(s_top[turn][w]));
         if (k) {
-            int reached = 0x7fffffff;
+            // the `bounding`-th largest of what the warps have reached
+            const int mine = s_reached[turn][lane % NW];
+            uint32_t larger = 0;
 #pragma unroll
-            for (int w = 0; w < NW; ++w)
-                if (w < bounding) reached = min(reached, s_reached[turn][w]);
-            bound = fmaxf(bound, rising_value(reached));
+            for (int w = 0; w < NW; ++w) {
+                const int other = s_reached[turn][w];
+                larger += other > mine || (other == mine && w < (int)(lane % NW));
+            }
+            const uint32_t who = __ballot_sync(0xffffffffu, larger == bounding - 1);
+            bound = fmaxf(bound, rising_value(__shfl_sync(0xffffffffu, mine, __ffs(who) - 1)));
         }
         raise(p, m);
         // y = x log2(e) - r with r = m log2(e) rounded: all e come out 2^slip too large, which is taken back below
@@ -392,36 +400,39 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
             p.d -= (e2 + e3 - slip * sum) * back * 0.6931471805599453f;
         }
         if (ordinary && warp_top >= xt) {
-            const uint32_t xt2 = pack_bf16x2(xt, xt);
-            uint32_t ahead2 = 0;  // two bf16 counts, at most 32 each
+            if constexpr (BF) {
+                // what lies before the target is ahead if it is larger than the number below xt
+                const uint32_t bits = __float_as_uint(xt) >> 16;
+                const uint32_t below = (bits & 0x7fffu) == 0 ? 0x8001u : bits & 0x8000u ? bits + 1 : bits - 1;
+                const uint32_t xt2 = bits * 0x10001u, below2 = below * 0x10001u;
+                uint32_t ahead2 = 0;  // two bf16 counts, at most 32 each
+                int col = first + (int)(v0 + threadIdx.x) * EPV;
+#pragma unroll 4
+                for (int v = 0; v < kVecs; ++v, col += T * EPV) {
+                    const uint4 y4 = x[v * T];
+                    const uint32_t than = col + EPV <= t ? below2 : xt2;
+                    ahead2 = add_bf16x2(ahead2, add_bf16x2(above_bf16x2(y4.x, than), above_bf16x2(y4.y, than)));
+                    ahead2 = add_bf16x2(ahead2, add_bf16x2(above_bf16x2(y4.z, than), above_bf16x2(y4.w, than)));
+                }
+                p.ahead += (uint32_t)(bf16_lo_to_f32(ahead2) + bf16_hi_to_f32(ahead2));
+            } else {
 #pragma unroll 2
-            for (int v = 0; v < kVecs; ++v) {
-                const uint4 y4 = x[v * T];
-                const uint32_t w[4] = {y4.x, y4.y, y4.z, y4.w};
-                const int col = first + (int)(v0 + v * T + threadIdx.x) * EPV;
-                if (col <= t && t < col + EPV) {
-#pragma unroll 1
-                    for (int i = 0; i < EPV; ++i) {
-                        const float e = picked<BF>(x + v * T, i);
-                        p.ahead += e > xt || (e == xt && col + i < t);
-                    }
-                } else if constexpr (BF) {
-                    if (col < t) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) ahead2 = add_bf16x2(ahead2, above_bf16x2<true>(w[i], xt2));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) ahead2 = add_bf16x2(ahead2, above_bf16x2<false>(w[i], xt2));
-                    }
-                } else {
+                for (int v = 0; v < kVecs; ++v) {
+                    const uint4 y4 = x[v * T];
+                    const int col = first + (int)(v0 + v * T + threadIdx.x) * EPV;
 #pragma unroll
                     for (int i = 0; i < EPV; ++i) {
-                        const float e = __uint_as_float(w[i]);
-                        p.ahead += col < t ? e >= xt : e > xt;
+                        const float e = element<false>(y4, i);
+                        p.ahead += col + EPV <= t ? e >= xt : e > xt;
                     }
                 }
             }
-            if constexpr (BF) p.ahead += (uint32_t)(bf16_lo_to_f32(ahead2) + bf16_hi_to_f32(ahead2));
+            // its own vector: what equals it and comes before it
+            const uint32_t at = (uint32_t)(t - first) / EPV - v0;  // vector of the step, if it is one
+            if (at < STEP && at % T == threadIdx.x) {
+#pragma unroll 1
+                for (uint32_t i = 0; i < (uint32_t)(t - first) % EPV; ++i) p.ahead += picked<BF>(x + at / T * T, i) == xt;
+            }
         }
         if (k && __any_sync(0xffffffffu, top >= bound && top > -CUDART_INF_F)) {
 #pragma unroll 1
@@ -625,7 +636,9 @@ cudaError_t launch_token_logprobs(const LogprobsLaunch& L, cudaStream_t stream) 
     a.status = L.status;
     a.cluster = 1;
     // As many warps as the row has 4 KB, up to 8; with too few rows to give every SM
-    // one, 8 warps and a cluster of CTAs for what is longer.
+    // one, 8 warps and a cluster of CTAs for what is longer.  Always 8 warps: 4096 rows
+    // of 1000 take 48 us instead of 12; always 1: 256 rows of 32768 48 instead of 13.
+    // Without clusters 8 rows of 131072 take 30 us instead of 10.
     const uint64_t parts = ((uint64_t)L.choices * (L.bf16 ? 2 : 4) + 4095) / 4096;
     uint32_t warps = 1;
     while (warps < kMostWarps && warps < parts) warps *= 2;
