@@ -16,6 +16,10 @@
 // RN(m/127) is taken the same way with RN(1/127), by one step, which is right for
 // all 2^23 mantissas (the tests go through them).  Rounding is the addition of
 // 1.5 * 2^23, whose low byte is the code; with |x| <= max|x| no clamp is needed.
+// 16 prompts of 1493 to 2048 tokens, 16 heads of 128: 75 us, 4.7 TB/s, 61 % of issue
+// slots; with the division instruction it took 156.  1023 tokens of 24 heads of 64:
+// 3 us.  Twice the rows a lane, for more loads in flight, cost more registers than
+// they hid.
 // A row that is not finite is divided one by one.  (Dividing only near half
 // integers does not pay: quotients of bf16 numbers fall on them too often.)
 #include "common.cuh"
@@ -274,7 +278,8 @@ cudaError_t launch_prompt_append(const PromptAppendLaunch& P, cudaStream_t strea
     a.capacity = P.arena->capacity;
     a.vec = P.vec;
     a.status = P.status;
-    // About 24 CTAs an SM where the prompts are long, at least one turn of rows each where they are short.
+    // About 24 CTAs an SM where the prompts are long, at least one turn of rows each where they are short.  64 tokens a
+    // CTA throughout: 1023 tokens 13 us instead of 3; one turn throughout: the 16 prompts 106 us instead of 75.
     const uint32_t turn = kThreads / (P.arena->head_dim / kE);
     uint32_t chunk = P.tokens / (12 * P.num_sms);
     chunk = chunk > (turn + a.heads - 1) / a.heads ? chunk : (turn + a.heads - 1) / a.heads;
