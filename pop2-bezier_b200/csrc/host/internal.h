@@ -132,7 +132,7 @@ struct AttnLaunch {
 //   PromptHeader                            @ 0
 //   seq_base  u32 [sequences + 1]     first uncut entry of each sequence
 //   entries   PromptEntry [max_entries]     longest first
-//   cuts      u32 [max_ctas]                first piece of each cut entry
+//   cuts      PromptEntry [max_ctas]        each cut entry
 //   acc       f32 [slots][slot_rows][head_dim]   partials of cut items
 //   ml        f32 [slots][slot_rows][2]          their maximum (log2 units), sum
 // An entry is cut only when its steps (prompt.cu) are more than `limit`, one and a
@@ -174,7 +174,7 @@ inline PromptWsLayout prompt_ws_layout(uint32_t sequences, uint32_t q_tokens, ui
     l.entries = off;
     off = align_up(off + sizeof(PromptEntry) * (size_t)l.max_entries, 256);
     l.cuts = off;
-    off = align_up(off + 4ull * max_ctas, 256);
+    off = align_up(off + sizeof(PromptEntry) * (size_t)max_ctas, 256);
     l.acc = off;
     off = align_up(off + 4ull * l.max_slots * l.slot_rows * head_dim, 256);
     l.ml = off;

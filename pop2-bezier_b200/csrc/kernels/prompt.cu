@@ -10,21 +10,22 @@ namespace {
 // ----------------------------------------------------------------- the plan
 //
 // One CTA, a thread an entry (up to 1024; a fixed 1024 took 0.7 us longer in small
-// batches); it is a chain of a few loads and barriers, 3 to 5 us, of which the launch
-// of the attention hides its own part.  Cuts every sequence into entries of 2 * tpt query tokens, counts
-// the steps each takes (a step is a key tile of both its query tiles, or two
+// batches); it is a chain of a few loads and barriers, 3 to 5 us, in which the
+// attention is launched.  Cuts every sequence into entries of 2 * tpt query tokens,
+// counts the steps each takes (a step is a key tile of both its query tiles, or two
 // key tiles where only one has rows), and writes them longest first (64 classes
 // of length), because the attention CTAs take items in this order as they
 // become free: the last ones taken are the shortest.  Where the whole batch has
 // fewer steps than it takes to keep every CTA busy with whole entries, entries of
 // more than one and a half times their share are cut into equal pieces along the
 // keys.  Pieces nearer to the share leave less room for the uneven last round (2048
-// causal tokens of 16 heads of 128: 43 us at 1.5, 51 at 1; 512 tokens at the end of
+// causal tokens of 16 heads of 128: 41 us at 1.5, 51 at 1; 512 tokens at the end of
 // 32768, 16 heads on 2: 134 and 208); longer ones leave SMs without work (172 at 2).
 // Uncut it takes 450 us, and one sequence of 8192, one head of 64, 109 against 38.
-// Nothing is cut where no entry has kCutSteps: partials and their merge take about
-// as long as three steps (768 tokens, 8 heads of 64, cut from 6 steps on: 20.5 us
-// against 19.8; 2000 keys of one token, cut: 21 against 30).
+// Nothing is cut where no entry has kCutSteps, or where the longest would lose less
+// than three: partials and their merge take about as long (768 tokens, 8 heads of 64,
+// cut from 6 steps on: 20.5 us against 19.8; 1023 tokens, 32 heads on 8 of 128, 6 steps
+// instead of 8: 34 against 29; one token over 2000 keys, 2 instead of 8: 20 against 29).
 constexpr uint32_t kPlanThreads = 1024;  // at most
 constexpr uint32_t kClasses = 64;
 constexpr uint32_t kBaseMax = 2048;  // sequences whose first entries are kept in shared memory
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
     PromptHeader* hdr = reinterpret_cast<PromptHeader*>(a.ws);
     uint32_t* seq_base = a.sequences <= kBaseMax ? base_s : reinterpret_cast<uint32_t*>(a.ws + a.l.seq_base);
     PromptEntry* entries = reinterpret_cast<PromptEntry*>(a.ws + a.l.entries);
-    uint32_t* cut_list = reinterpret_cast<uint32_t*>(a.ws + a.l.cuts);
+    PromptEntry* cut_list = reinterpret_cast<PromptEntry*>(a.ws + a.l.cuts);
     if (t == 0) longest = slots = cuts = 0;
     for (uint32_t c = t; c < kClasses; c += threads) hist[c] = 0;
     if (t < 32) warp_work[t] = 0;
@@ -155,7 +156,8 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
     for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
     const float share = __fdividef((float)all * a.kv_heads, a.l.max_ctas);  // to a few units of 2^-24, which is plenty
     const uint32_t most = longest;
-    const uint32_t limit = most < kCutSteps ? most : (uint32_t)fminf(fmaxf(2.f, ceilf(1.5f * share)), 1e9f);
+    const uint32_t piece = (uint32_t)fminf(fmaxf(2.f, ceilf(1.5f * share)), 1e9f);
+    const uint32_t limit = most < kCutSteps || most < piece + 3 ? most : piece;
     const float per_step = __fdividef((float)kClasses, most);
     // pieces of an entry and the class of their length
     auto cut = [&](const Whole& w, uint32_t& pieces) {
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const PlanArg
         p.slot0 = p.pad[0] = p.pad[1] = 0;
         if (pieces > 1) {
             p.slot0 = atomicAdd(&slots, pieces);
-            cut_list[atomicAdd(&cuts, 1u)] = at;
+            cut_list[atomicAdd(&cuts, 1u)] = p;
         }
         const uint32_t end = p.kv_end;
         for (uint32_t s = 0; s < pieces; ++s) {
@@ -497,12 +499,27 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) prompt_rows_ker
 //
 // A warp merges four rows side by side: out = sum_s 2^(m_s - m) acc_s / sum_s 2^(m_s - m) z_s over
 // its pieces, a lane in 8 taking every eighth piece's m and z, in an order that
-// does not depend on who finished first.  It is a chain of dependent loads (header,
-// cut, entry, maxima, partials), so rows run side by side: 8 MB of partials, from
-// L2, take about 4 us, one row at a time took 10.  Merging inside the attention
+// does not depend on who finished first.  It is a chain of loads (cut, then maxima
+// and partials), so rows run side by side: 8 MB of partials, from L2, take about 4 us,
+// one row at a time took 10.  Merging inside the attention
 // kernels, by the CTA that brings an entry's last piece, took 17 to 33 thousand
 // cycles.
 constexpr uint32_t kMergeWarps = 8, kMergeRows = 4;  // rows of a warp at a time
+
+// Here and now: not moved to where it is used.
+__device__ __forceinline__ PromptEntry load_entry(const PromptEntry* p) {
+    static_assert(sizeof(PromptEntry) == 48, "three vectors");
+    union {
+        uint32_t w[12];
+        PromptEntry e;
+    } u;
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+        asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(u.w[4 * i]), "=r"(u.w[4 * i + 1]), "=r"(u.w[4 * i + 2]), "=r"(u.w[4 * i + 3])
+                     : "l"(reinterpret_cast<const uint4*>(p) + i));
+    return u.e;
+}
 
 template <int D, bool BF>
 __global__ void __launch_bounds__(32 * kMergeWarps) prompt_merge_kernel(const __grid_constant__ PromptArgs a) {
@@ -512,16 +529,21 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prompt_merge_kernel(const __
     };
     const uint32_t lane = threadIdx.x & 31;
     const PromptHeader* hdr = reinterpret_cast<const PromptHeader*>(a.ws);
-    const PromptEntry* entries = reinterpret_cast<const PromptEntry*>(a.ws + a.l.entries);
-    const uint32_t* cuts = reinterpret_cast<const uint32_t*>(a.ws + a.l.cuts);
+    const PromptEntry* cuts = reinterpret_cast<const PromptEntry*>(a.ws + a.l.cuts);
     const float* acc = reinterpret_cast<const float*>(a.ws + a.l.acc);
     const float* ml = reinterpret_cast<const float*>(a.ws + a.l.ml);
+    const uint32_t rows = a.l.slot_rows, quads = rows / kMergeRows, sub = lane / 8, piece = lane % 8;
+    // The plan is complete before the attention lets this kernel start (prompt_tc.cu; prompt_rows_kernel lets it start at
+    // its end), so it is read before the wait.
+    const uint32_t n_cuts = hdr->n_cuts;
+    uint32_t i = blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+    PromptEntry next = load_entry(cuts + min(i / quads / a.kv_heads, a.l.max_ctas - 1));
     pdl_wait_primary();
-    const uint32_t groups = hdr->n_cuts * a.kv_heads, rows = a.l.slot_rows, quads = rows / kMergeRows;
-    const uint32_t sub = lane / 8, piece = lane % 8;
-    for (uint32_t i = blockIdx.x * kMergeWarps + (threadIdx.x >> 5); i < groups * quads; i += gridDim.x * kMergeWarps) {
+    while (i < n_cuts * a.kv_heads * quads) {
+        const PromptEntry e = next;
         const uint32_t row0 = i % quads * kMergeRows, head = i / quads % a.kv_heads;
-        const PromptEntry e = entries[cuts[i / quads / a.kv_heads]];
+        i += gridDim.x * kMergeWarps;
+        next = load_entry(cuts + min(i / quads / a.kv_heads, a.l.max_ctas - 1));
         auto token_of = [&](uint32_t row) {
             return e.tok0 + row / kPromptTileRows * a.tpt + row % kPromptTileRows / a.group;
         };
