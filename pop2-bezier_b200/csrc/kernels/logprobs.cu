@@ -22,11 +22,11 @@
 // Alternatives: with q = ceil(k / NW), take every warp's q-th largest lane maximum;
 // the ceil(k / q)-th largest of these is reached by at least k logits, so it is no
 // larger than the k-th best.  Only logits from the best such bound on are candidates
-// (on random rows one or two times k of a step's); they wait in a buffer until the
-// row ends or a warp has used half its share of it.  A candidate's place in the list is the number of
+// (on random rows one or two times k of a step's); they wait in a buffer a warp until
+// the row ends; a warp whose buffer is half full keeps its best k.  A candidate's place in the list is the number of
 // candidates ahead of it, which one thread each counts; the order in which they were
 // found does not matter.  Where a step leaves more candidates than the buffer holds
-// (long ties), the block takes the maximum k times instead.
+// (long ties), the block then takes the maximum k times instead.
 //
 // Bound by issue slots and the barrier of a step: 4096 rows of 32768 bf16 with 5
 // alternatives 81 us, 3.3 TB/s (maximum and sums alone 53, the rank 8, alternatives
@@ -178,21 +178,31 @@ __device__ __forceinline__ int rising(float x) {
 }
 __device__ __forceinline__ float rising_value(int k) { return __int_as_float(k ^ (k >> 31 & 0x7fffffff)); }
 
-// The list of the best 32 from the candidates and the list before it, by all of the block.
-__device__ __noinline__ void sort_candidates(const unsigned long long* cand, uint32_t count,
-                                             const unsigned long long* old, unsigned long long* list, uint32_t k) {
-    const uint32_t lane = threadIdx.x & 31;
-    const uint32_t before = __popc(__ballot_sync(0xffffffffu, lane < k && old[lane] != 0ull));
-    if (threadIdx.x < 32 && lane >= count + before) list[lane] = 0ull;
-    for (uint32_t j = threadIdx.x; j < count + before; j += blockDim.x) {
-        const unsigned long long mine = j < count ? cand[j] : old[j - count];
+// The list of the best 32 candidates, by all of the block; nothing is written beyond them.
+__device__ __noinline__ void sort_candidates(const unsigned long long* cand, uint32_t count, unsigned long long* list) {
+    for (uint32_t j = threadIdx.x; j < count; j += blockDim.x) {
+        const unsigned long long mine = cand[j];
         uint32_t place = 0;
 #pragma unroll 4
         for (uint32_t i = 0; i < count; ++i) place += cand[i] > mine;
-#pragma unroll 4
-        for (uint32_t i = 0; i < before; ++i) place += old[i] > mine;
         if (place < 32) list[place] = mine;
     }
+}
+
+// Keeps the best k of a warp's candidates, by the warp; returns how many there are.
+__device__ __noinline__ uint32_t keep_best(unsigned long long* cand, uint32_t count, uint32_t k) {
+    const uint32_t lane = threadIdx.x & 31;
+    const unsigned long long a = lane < count ? cand[lane] : 0ull, b = lane + 32 < count ? cand[lane + 32] : 0ull;
+    uint32_t place_a = 0, place_b = 0;
+    for (uint32_t i = 0; i < count; ++i) {
+        place_a += cand[i] > a;
+        place_b += cand[i] > b;
+    }
+    __syncwarp();
+    if (a && place_a < k) cand[place_a] = a;
+    if (b && place_b < k) cand[place_b] = b;
+    __syncwarp();
+    return min(count, k);
 }
 
 template <bool BF, int NW>
@@ -201,15 +211,15 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
     constexpr uint32_t T = 32 * NW, STEP = T * kVecs;  // vectors a CTA takes at a time
     constexpr int kLow = (int)0x807fffff;              // rising(-inf)
     extern __shared__ uint4 s_row[];                   // a step, vector v of thread t at v T + t
-    __shared__ int s_top[2][NW], s_reached[2][NW];
-    __shared__ unsigned long long s_cand[NW * kCandidates], s_list[2][32], s_best[NW];
-    __shared__ uint32_t s_count;
+    __shared__ int s_top[NW];
+    __shared__ volatile int s_reached[NW];             // only rises: any value read is a bound
+    __shared__ unsigned long long s_cand[NW * kCandidates], s_all[NW * kCandidates], s_list[32], s_best[NW];
+    __shared__ uint32_t s_found[NW];
     __shared__ Part s_part[NW], s_cta;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t row = a.cluster > 1 ? blockIdx.x / a.cluster : blockIdx.x, part = a.cluster > 1 ? cluster_rank() : 0u;
     const uint32_t k = a.top;
-    if (threadIdx.x == 0) s_count = 0;
-    if (warp == 0) s_list[0][lane] = 0ull;
+    if (warp == 0) s_list[lane] = 0ull;
     const uint32_t q = (k + NW - 1) / NW;  // lane maxima of a warp that have to reach the bound
     const uint32_t bounding = k ? (k + q - 1) / q : 0u;
     pdl_wait_primary();
@@ -267,13 +277,11 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
 
     Part p{-CUDART_INF_F, 0.f, 0.f, 0.f, 0u};
     const uint4* x = s_row + threadIdx.x;
-    uint32_t turn = 0;     // steps take turns at what the warps tell each other
-    uint32_t current = 0;  // which of the two lists is the last one
-    uint32_t found = 0;    // candidates of the warp
+    unsigned long long* cand = s_cand + warp * kCandidates;
+    uint32_t found = 0;  // candidates of the warp
     float bound = -CUDART_INF_F;
     bool over = false;  // candidates did not fit: the list is found in the row again
-    __syncthreads();
-    for (uint32_t v0 = part * STEP; v0 < vectors; v0 += stride, turn ^= 1) {
+    for (uint32_t v0 = part * STEP; v0 < vectors; v0 += stride) {
         cp_async_wait_all();
         float top = -CUDART_INF_F;
         if constexpr (BF) {
@@ -303,30 +311,27 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
                     reached = __reduce_max_sync(0xffffffffu, left >> lane & 1u ? key : kLow);
                 }
             }
-            if (lane == 0) s_reached[turn][warp] = reached;
+            if (lane == 0 && (v0 == part * STEP || reached > s_reached[warp])) s_reached[warp] = reached;
         }
-        if (lane == 0) s_top[turn][warp] = warp_key;
-        if (__syncthreads_or(found > kCandidates / 2)) {  // a warp has used half its share of the buffer
-            over = __syncthreads_or(found > kCandidates) || over;
-            if (!over) sort_candidates(s_cand, s_count, s_list[current], s_list[current ^ 1], k);
+        float m = fmaxf(p.m, warp_top);
+        if (v0 == part * STEP) {  // the warps start from one maximum and bound, and then go their own ways
+            if (lane == 0) s_top[warp] = warp_key;
             __syncthreads();
-            if (threadIdx.x == 0) s_count = 0;
-            found = 0;
-            current ^= 1;
-            const unsigned long long kth = s_list[current][k - 1];
-            if (!over && kth) bound = fmaxf(bound, order_value(kth));
-            __syncthreads();
-        }
-        float m = p.m;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) m = fmaxf(m, rising_value(s_top[turn][w]));
+            for (int w = 0; w < NW; ++w) m = fmaxf(m, rising_value(s_top[w]));
+        }
         if (k) {
+            if (found > kCandidates / 2) {
+                over = over || found > kCandidates;
+                found = keep_best(cand, min(found, kCandidates), k);
+                if (found == k) bound = fmaxf(bound, order_value(cand[k - 1]));
+            }
             // the `bounding`-th largest of what the warps have reached
-            const int mine = s_reached[turn][lane % NW];
+            const int mine = s_reached[lane % NW];
             uint32_t larger = 0;
 #pragma unroll
             for (int w = 0; w < NW; ++w) {
-                const int other = s_reached[turn][w];
+                const int other = __shfl_sync(0xffffffffu, mine, w);
                 larger += other > mine || (other == mine && w < (int)(lane % NW));
             }
             const uint32_t who = __ballot_sync(0xffffffffu, larger == bounding - 1);
@@ -448,13 +453,11 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
                     have |= (e >= bound && e > -CUDART_INF_F ? 1u : 0u) << i;
                 }
                 for (uint32_t who; (who = __ballot_sync(0xffffffffu, have != 0)) != 0; have &= have - 1) {
-                    uint32_t at = 0;
+                    const uint32_t at = found + __popc(who & ((1u << lane) - 1u));
                     found += __popc(who);
-                    if (lane == 0 && found <= kCandidates) at = atomicAdd(&s_count, __popc(who));
-                    at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
-                    if (have && found <= kCandidates) {
+                    if (have && at < kCandidates) {
                         const int i = __ffs(have) - 1;
-                        s_cand[at] = order_of(picked<BF>(x + v * T, i), (uint32_t)(col + i));
+                        cand[at] = order_of(picked<BF>(x + v * T, i), (uint32_t)(col + i));
                     }
                 }
             }
@@ -462,13 +465,29 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
         if (v0 + stride < vectors) fetch(v0 + stride);
     }
     if (k) {
-        over = __syncthreads_or(found > kCandidates) || over;
+        // What has fallen behind the bound goes; the rest of all warps, one after another.
+        over = over || found > kCandidates;
+        found = min(found, kCandidates);
+        __syncwarp();
+        const bool has_a = lane < found && order_value(cand[lane]) >= bound;
+        const bool has_b = lane + 32 < found && order_value(cand[lane + 32]) >= bound;
+        const uint32_t as = __ballot_sync(0xffffffffu, has_a), bs = __ballot_sync(0xffffffffu, has_b);
+        const uint32_t below = (1u << lane) - 1u;
+        if (lane == 0) s_found[warp] = __popc(as) + __popc(bs);
+        over = __syncthreads_or(over);
         if (!over) {
-            sort_candidates(s_cand, s_count, s_list[current], s_list[current ^ 1], k);
-            current ^= 1;
-        } else {
-            unsigned long long* list = s_list[current];
+            uint32_t from = 0, all = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                from += w < (int)warp ? s_found[w] : 0u;
+                all += s_found[w];
+            }
+            if (has_a) s_all[from + __popc(as & below)] = cand[lane];
+            if (has_b) s_all[from + __popc(as) + __popc(bs & below)] = cand[lane + 32];
             __syncthreads();
+            sort_candidates(s_all, all, s_list);
+        } else {
+            unsigned long long* list = s_list;
             unsigned long long prev = ~0ull;
             for (uint32_t j = 0; j < k; ++j) {
                 unsigned long long best = 0;
@@ -515,7 +534,11 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
     if (lane == 0) s_part[warp] = p;
     __syncthreads();
     if (warp == 0 && NW > 1) {
-        p = lane < NW ? s_part[lane] : Part{p.m, 0.f, 0.f, 0.f, 0u};
+        p = lane < NW ? s_part[lane] : Part{-CUDART_INF_F, 0.f, 0.f, 0.f, 0u};
+        float m = p.m;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        raise(p, m);
 #pragma unroll
         for (int o = NW / 2; o; o >>= 1) {
             p.s += __shfl_xor_sync(0xffffffffu, p.s, o);
@@ -526,7 +549,6 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
     }
     if (NW == (int)kMostWarps && a.cluster > 1) {
         if (threadIdx.x == 0) s_cta = p;
-        if (warp == 0 && current) s_list[0][lane] = s_list[1][lane];  // peers look at the first
         cluster_sync();
         if (part == 0) {
             if (warp == 0) {  // lane r fetches CTA r's part
@@ -550,7 +572,7 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
                 }
             }
             if (k && warp < a.cluster && lane < k) {  // a warp fetches a CTA's list
-                const uint32_t* peer = reinterpret_cast<const uint32_t*>(&s_list[0][lane]);
+                const uint32_t* peer = reinterpret_cast<const uint32_t*>(&s_list[lane]);
                 const unsigned long long l = ld_peer(peer, warp), h = ld_peer(peer + 1, warp);
                 s_cand[warp * k + lane] = h << 32 | l;
             }
@@ -558,14 +580,10 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
         cluster_sync();  // the peers' shared memory has been read
         if (part != 0) return;
         if (k) {
-            if (warp == 0) {
-                s_list[0][lane] = 0ull;
-                s_list[1][lane] = 0ull;
-            }
+            if (warp == 0) s_list[lane] = 0ull;
             __syncthreads();
             // missing entries are 0 and land behind the others, where the list is 0
-            sort_candidates(s_cand, a.cluster * k, s_list[0], s_list[1], k);
-            current = 1;
+            sort_candidates(s_cand, a.cluster * k, s_list);
             __syncthreads();
         }
     }
@@ -581,7 +599,7 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
         a.rank[row] = inside ? p.ahead : (uint32_t)n;
     }
     if (lane < k) {
-        const unsigned long long o = s_list[current][lane];
+        const unsigned long long o = s_list[lane];
         a.top_ids[(uint64_t)row * k + lane] = o ? ~(uint32_t)o : 0xffffffffu;
         float lp = -CUDART_INF_F;
         if (o) lp = nothing ? CUDART_NAN_F : (order_value(o) - p.m) - lse;
