@@ -13,27 +13,31 @@
 // A thread copies 8 vectors of 16 bytes into shared memory (cp.async) and looks at
 // them several times (maximum, sums, rank, alternatives) in short loops: nothing
 // waits for another thread's copies, and the loops stay in the instruction cache,
-// which the same code unrolled over registers did not (4096 rows of 32768, with
-// the bound of that time: 154 us against 95).  One buffer a CTA leaves room for five CTAs an SM, which hide the
-// copies better than a second buffer with three (117 us).  NW warps take 4 KB each of a
-// row; a longer row is taken in steps, with one barrier each, or by a cluster of
-// up to 8 CTAs that merge through their shared memory, when there are few rows.
+// which the same code unrolled over registers did not (4096 rows of 32768, with the
+// bound of that time: 154 us against 95).  One buffer a CTA leaves room for five CTAs
+// an SM, which hide the copies better than a second buffer with three (117 us).  NW
+// warps take 4 KB each of a row; a longer row is taken in steps, with a barrier after
+// the first, or by a cluster of up to 8 CTAs that merge through their shared memory,
+// when there are few rows.
 //
 // Alternatives: with q = ceil(k / NW), take every warp's q-th largest lane maximum;
 // the ceil(k / q)-th largest of these is reached by at least k logits, so it is no
 // larger than the k-th best.  Only logits from the best such bound on are candidates
 // (on random rows one or two times k of a step's); they wait in a buffer a warp until
-// the row ends; a warp whose buffer is half full keeps its best k.  A candidate's place in the list is the number of
-// candidates ahead of it, which one thread each counts; the order in which they were
-// found does not matter.  Where a step leaves more candidates than the buffer holds
-// (long ties), the block then takes the maximum k times instead.
+// the row ends; a warp whose buffer is half full keeps its best k.  A candidate's
+// place in the list is the number of candidates ahead of it, which one thread each
+// counts; the order in which they were found does not matter.  Where a step leaves
+// more candidates than the buffer holds (long ties, sorted rows), the block then takes
+// the maximum k times instead: 4096 rows of 32768 in order take 650 us with 5
+// alternatives.  Searching them with a better bound takes 450, but its registers cost
+// random rows 6 to 30 % (81 to 99 us instead of 76).
 //
-// Bound by issue slots and the barrier of a step: 4096 rows of 32768 bf16 with 5
-// alternatives 81 us, 3.3 TB/s (maximum and sums alone 53, the rank 8, alternatives
-// 20); few rows by latency: 8 of 131072 with 20 alternatives 12 us; 2304 windows of
-// up to 1024 f32 9 us.  With the least of the first ceil(k / q) warps' values as the
-// bound there are twice the candidates: 100 us.  Candidates pushed lane by lane, with
-// an atomic each, instead of warp by warp: 98 us.
+// Bound by issue slots and latency: 4096 rows of 32768 bf16 with 5 alternatives 76 us,
+// 3.5 TB/s (maximum and sums alone 51, the rank 8, alternatives 18); 2048 of 131072
+// 121 us, 4.4 TB/s; few rows by latency: 8 of 131072 with 20 alternatives 10 us; 2304
+// windows of up to 1024 f32 8 us.  With a barrier a step 81 and 140 us; with the least
+// of the first ceil(k / q) warps' values as the bound, twice the candidates, 100.
+// Candidates pushed lane by lane, with an atomic each, instead of warp by warp: 98.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -192,6 +196,7 @@ __device__ __noinline__ void sort_candidates(const unsigned long long* cand, uin
 // Keeps the best k of a warp's candidates, by the warp; returns how many there are.
 __device__ __noinline__ uint32_t keep_best(unsigned long long* cand, uint32_t count, uint32_t k) {
     const uint32_t lane = threadIdx.x & 31;
+    __syncwarp();  // other lanes' candidates
     const unsigned long long a = lane < count ? cand[lane] : 0ull, b = lane + 32 < count ? cand[lane + 32] : 0ull;
     uint32_t place_a = 0, place_b = 0;
     for (uint32_t i = 0; i < count; ++i) {

@@ -147,6 +147,18 @@ def test_ties_go_to_the_lower_column(pp, cuda, choices, dtype):
     check(pp, x.to(dtype), t, 32)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("rows,choices", [(3, 140001), (200, 40000), (40, 3000)])
+@pytest.mark.parametrize("top", [1, 5, 32])
+def test_rows_in_order(pp, cuda, top, rows, choices, dtype):
+    """Rising, falling and half-sorted rows: every column, or none, is a candidate when it comes."""
+    x, t = make(cuda, rows, choices, dtype, choices + top)
+    x[0::3] = x[0::3].sort(1).values
+    x[1::3] = x[1::3].sort(1, descending=True).values
+    x[2::3, choices // 2:] = x[2::3, choices // 2:].sort(1).values
+    check(pp, x, t, top)
+
+
 def test_a_nearly_certain_token_keeps_its_digits(pp, cuda):
     """logprob about -1e-9: 1 + s would round it to 0 in f32."""
     x = torch.zeros(4, 1000, device=cuda)
