@@ -36,6 +36,7 @@ pub const PP_DEV_LENGTH_RANGE: u32 = 0x4;
 pub const PP_DEV_WAIT_TIMEOUT: u32 = 0x8;
 pub const PP_DEV_POSITION_RANGE: u32 = 0x10;
 pub const PP_DEV_WINDOW_RANGE: u32 = 0x20;
+pub const PP_DEV_PLAN_MISMATCH: u32 = 0x40;
 
 pub const PP_ATTN_PLAN_READY: u32 = 0x1;
 pub const PP_ATTN_PREFETCH_HISTORY: u32 = 0x2;

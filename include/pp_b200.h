@@ -57,6 +57,7 @@ extern "C" {
 #define PP_DEV_WAIT_TIMEOUT 0x8u     /* a bounded pipeline wait gave up: output undefined */
 #define PP_DEV_POSITION_RANGE 0x10u  /* RoPE position >= max_context: row not written */
 #define PP_DEV_WINDOW_RANGE 0x20u    /* window of legal tokens outside the choices: row outputs are NaN */
+#define PP_DEV_PLAN_MISMATCH 0x40u   /* PP_ATTN_PLAN_READY on a workspace without this prompt's plan: nothing written */
 
 /* Geometry of a caller-owned int8 KV arena for one layer, in the reference's
  * batch-arena layout (app/src/model/cache.rs:301-478, int8_cache.rs:326-359):
@@ -275,8 +276,10 @@ size_t pp_b200_prompt_workspace_size(const PpPrompt* prompt);
 /* The work list of these sequences: tiles of query rows, longest first, and
  * cut along the keys where there are too few of them to fill the GPU.  Every
  * layer of a step reuses it with PP_ATTN_PLAN_READY (same geometry, strides
- * apart, same max_ctas and same lengths).  q, k and v may be NULL here.  The
- * workspace belongs to one call at a time.
+ * apart, same max_ctas and same lengths).  The workspace records the geometry:
+ * a call that finds another one there, or no plan, writes nothing and sets
+ * PP_DEV_PLAN_MISMATCH; the lengths are the caller's to keep.  q, k and v may be
+ * NULL here.  The workspace belongs to one call at a time.
  * status (nullable): PP_DEV_LENGTH_RANGE. */
 int32_t pp_b200_plan_prompt(const PpPrompt* prompt, const uint32_t* q_starts, const uint32_t* kv_starts,
                             void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
@@ -284,7 +287,8 @@ int32_t pp_b200_plan_prompt(const PpPrompt* prompt, const uint32_t* q_starts, co
 /* Attention of every query token over its own sequence, scores, softmax and
  * sums in f32.  out: [q_tokens, heads, head_dim] of the prompt's dtype, dense,
  * not overlapping q, k or v.
- * status (nullable): PP_DEV_LENGTH_RANGE, PP_DEV_WAIT_TIMEOUT. */
+ * status (nullable): PP_DEV_LENGTH_RANGE, PP_DEV_WAIT_TIMEOUT,
+ * PP_DEV_PLAN_MISMATCH. */
 int32_t pp_b200_prompt_attention(const PpPrompt* prompt, const uint32_t* q_starts, const uint32_t* kv_starts,
                                  void* out, void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
 

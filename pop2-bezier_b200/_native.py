@@ -25,6 +25,7 @@ DEV_LENGTH_RANGE = 0x4
 DEV_WAIT_TIMEOUT = 0x8
 DEV_POSITION_RANGE = 0x10
 DEV_WINDOW_RANGE = 0x20
+DEV_PLAN_MISMATCH = 0x40
 
 ATTN_PLAN_READY = 0x1
 ATTN_PREFETCH_HISTORY = 0x2

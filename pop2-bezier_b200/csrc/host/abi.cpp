@@ -680,6 +680,7 @@ const char* pp_b200_status_message(uint32_t bits) {
     if (bits & PP_DEV_LENGTH_RANGE) return "INT8 attention lengths differ: length exceeds capacity (row output is NaN)";
     if (bits & PP_DEV_POSITION_RANGE) return "graph QKV/RoPE position exceeds the RoPE table (row not written)";
     if (bits & PP_DEV_WINDOW_RANGE) return "token window outside the head's choices (row outputs are NaN)";
+    if (bits & PP_DEV_PLAN_MISMATCH) return "prompt workspace holds no plan of this geometry (nothing written)";
     return "unknown device status";
 }
 

@@ -142,7 +142,7 @@ struct PromptHeader {
     uint32_t n_items;  // entries * kv_heads
     uint32_t next;     // next item to hand out beyond the grid's first ones (zero between calls)
     uint32_t n_cuts;   // entries cut along their keys
-    uint32_t pad[5];
+    uint32_t key[5];   // what the plan was made for (prompt_plan_key)
 };
 
 struct PromptEntry {
@@ -181,6 +181,16 @@ inline PromptWsLayout prompt_ws_layout(uint32_t sequences, uint32_t q_tokens, ui
     off = align_up(off + 8ull * l.max_slots * l.slot_rows, 256);
     l.total = off;
     return l;
+}
+
+// The geometry that a plan depends on, and that offsets into its workspace do.
+// Never 0 in the last word: a cleared workspace holds no plan.
+inline void prompt_plan_key(const PpPrompt& g, uint32_t max_ctas, uint32_t (&key)[5]) {
+    key[0] = g.sequences;
+    key[1] = g.q_tokens;
+    key[2] = g.kv_tokens;
+    key[3] = g.heads | g.kv_heads << 16;  // at most 65535 each
+    key[4] = max_ctas | (g.causal ? 1u << 20 : 0u) | (g.head_dim == 128 ? 1u << 21 : 0u) | 1u << 31;
 }
 
 struct PromptLaunch {

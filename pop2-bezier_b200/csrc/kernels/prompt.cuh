@@ -34,8 +34,23 @@ struct PromptArgs {
     uint32_t causal;
     float scale_log2;
     uint32_t vec;  // 16-byte loads of q, k and v rows are aligned
+    uint32_t key[5];  // of the plan that the workspace has to hold
     uint32_t* status;
 };
+
+// The plan's header, if the plan is one of this geometry; otherwise one without
+// items, and PP_DEV_PLAN_MISMATCH from the thread that reports.
+__device__ __forceinline__ PromptHeader plan_header(const PromptArgs& a, bool report) {
+    PromptHeader h = *reinterpret_cast<const PromptHeader*>(a.ws);
+    uint32_t differ = 0;
+#pragma unroll
+    for (int i = 0; i < 5; ++i) differ |= h.key[i] ^ a.key[i];
+    if (differ) {
+        h.n_items = h.n_cuts = 0;
+        if (report && a.status) atomicOr(a.status, PP_DEV_PLAN_MISMATCH);
+    }
+    return h;
+}
 
 __device__ __forceinline__ uint32_t prompt_visible(const PromptEntry& e, uint32_t token, uint32_t causal) {
     if (!causal) return e.nk;

@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ------------------------------------------------ items and loads
             PromptHeader* hdr = reinterpret_cast<PromptHeader*>(a.ws);
             const PromptEntry* entries = reinterpret_cast<const PromptEntry*>(a.ws + a.l.entries);
-            const uint32_t n_items = hdr->n_items;
+            const uint32_t n_items = plan_header(a, blockIdx.x == 0).n_items;
             const uint32_t q_bytes = a.group * a.tpt * 128 * (D / 64);
             uint32_t stage = 0, phase = 0, kv = 0, q_use0 = 0, q_use1 = 0, idx = blockIdx.x;
             bool ok = true;

@@ -172,7 +172,9 @@ def plan_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts: tor
                 status: torch.Tensor | None = None) -> None:
     """Writes the work list of these sequences into `workspace`, for the
     prompt_attention calls with plan_ready=True that follow: every layer of a
-    prefill has the same shapes and lengths."""
+    prefill has the same shapes and lengths.  A call of another shape,
+    causality, max_ctas or number of sequences writes nothing and sets
+    DEV_PLAN_MISMATCH in its status word."""
     n = _starts(q_starts, None, q.device)
     if kv_starts is not None:
         _starts(kv_starts, n, q.device)
@@ -207,8 +209,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts
     later chunk of a prompt, or a single token).  A query that sees no key
     gives NaN; rows of `out` that no sequence holds are left as they were.
     softmax_scale 0: 0.125 at d = 64, 1/sqrt(d) otherwise.  A status word gets
-    DEV_LENGTH_RANGE when the starts decrease or pass the tensors' ends (then
-    nothing is written)."""
+    DEV_LENGTH_RANGE when the starts decrease or pass the tensors' ends, and
+    DEV_PLAN_MISMATCH when plan_ready finds no plan of this geometry in the
+    workspace (in both cases nothing is written)."""
     n = _starts(q_starts, None, q.device)
     if kv_starts is not None:
         _starts(kv_starts, n, q.device)
