@@ -278,7 +278,8 @@ size_t pp_b200_prompt_workspace_size(const PpPrompt* prompt);
  * layer of a step reuses it with PP_ATTN_PLAN_READY (same geometry, strides
  * apart, same max_ctas and same lengths).  The workspace records the geometry:
  * a call that finds another one there, or no plan, writes nothing and sets
- * PP_DEV_PLAN_MISMATCH; the lengths are the caller's to keep.  q, k and v may be
+ * PP_DEV_PLAN_MISMATCH, as does one after a call that ended with
+ * PP_DEV_WAIT_TIMEOUT; the lengths are the caller's to keep.  q, k and v may be
  * NULL here.  The workspace belongs to one call at a time.
  * status (nullable): PP_DEV_LENGTH_RANGE. */
 int32_t pp_b200_plan_prompt(const PpPrompt* prompt, const uint32_t* q_starts, const uint32_t* kv_starts,

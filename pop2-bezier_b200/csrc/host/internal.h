@@ -140,9 +140,9 @@ struct AttnLaunch {
 // limit pieces: at most 2 max_ctas slots and max_ctas cut items, kv_heads included.
 struct PromptHeader {
     uint32_t n_items;  // entries * kv_heads
-    uint32_t next;     // next item to hand out beyond the grid's first ones (zero between calls)
+    uint32_t next;     // next item to hand out beyond the grid's first ones (zero between calls, unless one gave up)
     uint32_t n_cuts;   // entries cut along their keys
-    uint32_t key[5];   // what the plan was made for (prompt_plan_key)
+    uint32_t key[5];   // what the plan was made for (prompt_plan_key); the last word is 0 after a call that gave up
 };
 
 struct PromptEntry {

@@ -178,6 +178,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     auto give_up = [&] {
         *abort = 1;
+        // `next` stays where it is, for the list is not handed out to its end: no plan for later calls
+        *reinterpret_cast<volatile uint32_t*>(&reinterpret_cast<PromptHeader*>(a.ws)->key[4]) = 0;
         if (a.status) atomicOr(a.status, PP_DEV_WAIT_TIMEOUT);
     };
     // One thread's wait.

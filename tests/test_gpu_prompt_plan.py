@@ -69,6 +69,28 @@ def test_a_workspace_without_a_plan_is_refused(pp, cuda, fill, dtype):
     assert "plan" in pp._native.status_message(int(status))
 
 
+def test_a_plan_is_void_after_a_call_that_gave_up(pp, cuda):
+    """Such a call leaves the counter of its list somewhere in the list (word 1 of the workspace) and clears the last
+    word of the geometry (word 7): later calls write nothing, instead of a part of their rows, until the next plan."""
+    q, k, v = tensors(cuda, 300, 3000, 4, 2, 64, torch.bfloat16)
+    fa = pp.fused_attention
+    qs, ks = starts_of([300], cuda), starts_of([3000], cuda)
+    ws = fa.prompt_workspace(q, k, v, 1)
+    fa.plan_prompt(q, k, v, qs, ws, kv_starts=ks)
+    header = ws[:32].view(torch.int32)
+    assert int(header[0]) > 1 and int(header[1]) == 0 and int(header[7]) != 0
+    header[1], header[7] = 1, 0
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    for _ in range(2):
+        out = torch.full_like(q, 7.0)
+        fa.prompt_attention(q, k, v, qs, kv_starts=ks, workspace=ws, plan_ready=True, out=out, status=status.zero_())
+        assert int(status) == pp._native.DEV_PLAN_MISMATCH and (out == 7).all()
+    fa.plan_prompt(q, k, v, qs, ws, kv_starts=ks)
+    fa.prompt_attention(q, k, v, qs, kv_starts=ks, workspace=ws, plan_ready=True, out=out, status=status.zero_())
+    assert int(status) == 0
+    check(out, q, k, v, [300], [3000], True)
+
+
 @BOTH
 def test_a_plan_serves_other_strides_and_types(pp, cuda, dtype):
     """The work list depends on shapes and lengths alone."""
