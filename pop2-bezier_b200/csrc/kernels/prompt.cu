@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prompt_merge_kernel(const __
 #pragma unroll
                 for (int c = 0; c < C; c += 2)
                     reinterpret_cast<uint32_t*>(a.out)[(at + c) / 2] = pack_bf16x2(o[u].f[c], o[u].f[c + 1]);
-                if (a.vec && zu != 0.f && __any_sync(0xffffffffu, !(chk == 0.f))) redo_row<D>(a, e, head, token, g);
+                if (a.vec && zu != 0.f && zu == zu && __any_sync(0xffffffffu, !(chk == 0.f))) redo_row<D>(a, e, head, token, g);
             } else {
                 *reinterpret_cast<Lane*>(reinterpret_cast<float*>(a.out) + at) = o[u];
             }

@@ -28,7 +28,7 @@
 // Keys that a row does not see get score -inf, hence P = 0, but 0 * v is not 0
 // where v is NaN or infinite (padding, later tokens of the same tile).  Such a
 // row ends up not finite, and its warp computes it again from the keys that it
-// does see.
+// does see, unless these explain it (prompt.cuh).
 //
 // What bounds it: at head_dim 128 the chain of a tile (S, softmax, P V), of which
 // two run side by side: the softmax of a key tile takes about 1850 cycles and the
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + __uint_as_float(x[i]) * f1);
                 }
             };
-            uint32_t again = 0;  // rows of this warp that are not finite though they see keys
+            uint32_t again = 0;  // rows of this warp that are not finite, though they see keys and their sum of P is a number
             const uint32_t warp_row = (warp & 3) * 32;
             auto out_row = [&](uint32_t row) {
                 return reinterpret_cast<__nv_bfloat16*>(a.out) +
@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                again = __ballot_sync(0xffffffffu, live && lim > 0 && !(chk == 0.f));
+                again = __ballot_sync(0xffffffffu, live && lim > 0 && z == z && !(chk == 0.f));
             } else {
                 // partial of this piece, for prompt_merge_kernel
                 auto slot_row = [&](uint32_t s, uint32_t row) {
