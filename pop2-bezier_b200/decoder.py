@@ -304,7 +304,7 @@ class SyntheticDecoder:
         H, d, tokens = cfg.heads, cfg.head_dim, sum(lengths)
         if len(lengths) != self.branches or min(lengths) < 0 or max(lengths) > min(self.capacity, cfg.max_context):
             raise N.PreconditionError("prefill needs one length a branch, within the arena and the RoPE table")
-        if tuple(x.shape) != (tokens, cfg.width) or x.dtype != self.dtype or x.device != self.device \
+        if tuple(x.shape) != (tokens, cfg.width) or x.dtype != self.dtype or x.device != self.final_norm.device \
                 or not x.is_contiguous():
             raise N.PreconditionError("prefill needs dense embeddings [sum(lengths), width] of the model's type")
         if tokens == 0:
