@@ -154,6 +154,12 @@ class PreconditionError(ValueError):
     """Status 1: invalid geometry or argument; nothing was launched."""
 
 
+def check_u32(*sizes: int) -> None:
+    """Refuses sizes that the C ABI's u32 does not hold: ctypes would drop their upper bits."""
+    if min(sizes) < 0 or max(sizes) > 0xFFFFFFFF:
+        raise PreconditionError(f"a size of {sizes} is not in 0 .. 2^32 - 1")
+
+
 class InvalidOutputError(RuntimeError):
     """Status 2: a device check found invalid data."""
 

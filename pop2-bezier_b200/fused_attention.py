@@ -149,6 +149,7 @@ def prompt_struct(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sequences: 
             or k.dtype != dt or v.dtype != dt or heads == 0 or kv_heads == 0 or heads % kv_heads or heads > 64 * kv_heads \
             or qs[2] != 1 or ks[2] != 1 or vs[2] != 1:
         raise N.PreconditionError(_MSG_PROMPT)
+    N.check_u32(sequences, tokens, kv_tokens, max_ctas)
     return N.PpPrompt(_PROMPT_BYTES, sequences, heads, kv_heads, d, code, tokens, kv_tokens, 1 if causal else 0,
                       softmax_scale, N.ATTN_PLAN_READY if plan_ready else 0, max_ctas, qs[0], qs[1], ks[0], ks[1], vs[0],
                       vs[1], q.data_ptr(), k.data_ptr(), v.data_ptr())

@@ -72,6 +72,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0,
     if logits.dim() != 2 or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise N.PreconditionError("token logprobs need logits [rows, choices] with contiguous rows and a nonempty head")
     rows, choices = logits.shape
+    N.check_u32(rows, choices)
     if targets.dim() != 1 or targets.numel() != rows or targets.dtype != torch.int32 or not targets.is_contiguous():
         raise N.PreconditionError("token logprobs need one contiguous I32 target a row")
     if bounds is not None and (bounds.numel() != 2 * rows or bounds.dtype not in (torch.int32, torch.uint32)
