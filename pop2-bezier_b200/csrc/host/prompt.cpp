@@ -103,7 +103,10 @@ int32_t pp_b200_prompt_attention(const PpPrompt* prompt, const uint32_t* q_start
                                "prompt_attention");
     if (s) return s;
     if (L.g.flags & ~PP_ATTN_PLAN_READY) return fail_fmt(PP_STATUS_PRECONDITION, "prompt_attention: unknown flags 0x%x", L.g.flags);
-    if (L.g.q_tokens == 0) return PP_STATUS_OK;  // no rows
+    if (L.g.q_tokens == 0)  // no rows, but starts that the plan checks
+        return L.g.flags & PP_ATTN_PLAN_READY
+                   ? PP_STATUS_OK
+                   : pp::cuda_status(pp::launch_prompt_plan(L, (cudaStream_t)stream), "prompt plan launch");
     if (!out || !aligned(out, 16)) return fail_fmt(PP_STATUS_PRECONDITION, "prompt_attention: out must be 16-byte aligned");
     L.out = out;
     const uint64_t elem = L.g.dtype == PP_DTYPE_F32 ? 4 : 2;
@@ -159,9 +162,9 @@ int32_t pp_b200_prompt_append(const PpKvArena* arena, const void* k, const void*
         return fail_fmt(PP_STATUS_PRECONDITION, "prompt_append: starts, offsets and status must be 4-byte aligned");
     pp::PromptAppendLaunch P{};
     if ((s = pp::device_sms(&P.num_sms))) return s;
-    if (tokens == 0) return PP_STATUS_OK;  // nothing to append
+    if (tokens == 0 && !status) return PP_STATUS_OK;  // nothing to append, and nowhere to report bad starts
     const uint64_t elem = dtype == PP_DTYPE_F32 ? 4 : 2;
-    if (!k || !v || !aligned(k, elem) || !aligned(v, elem))
+    if ((tokens && (!k || !v)) || !aligned(k, elem) || !aligned(v, elem))
         return fail_fmt(PP_STATUS_PRECONDITION, "prompt_append: NULL or misaligned K/V");
     P.arena = arena;
     P.k = k;

@@ -284,7 +284,7 @@ cudaError_t launch_prompt_append(const PromptAppendLaunch& P, cudaStream_t strea
     uint32_t chunk = P.tokens / (12 * P.num_sms);
     chunk = chunk > (turn + a.heads - 1) / a.heads ? chunk : (turn + a.heads - 1) / a.heads;
     a.chunk = chunk < kMaxChunk ? chunk : kMaxChunk;
-    const dim3 grid((P.tokens + a.chunk - 1) / a.chunk, 2);
+    const dim3 grid(P.tokens ? (P.tokens + a.chunk - 1) / a.chunk : 1, 2);  // without tokens the starts are checked
     if (P.arena->head_dim == 128)
         return P.bf16 ? launch_pdl(prompt_append_kernel<128, true>, grid, dim3(kThreads), stream, a)
                       : launch_pdl(prompt_append_kernel<128, false>, grid, dim3(kThreads), stream, a);

@@ -1,4 +1,4 @@
-"""Arguments of the prompt operators that only Python sees: sizes beyond the C ABI's."""
+"""Arguments of the prompt operators at their ends: sizes beyond 32 bits, and none."""
 from __future__ import annotations
 
 import pytest
@@ -36,3 +36,34 @@ def test_sizes_beyond_32_bits_are_refused(pp, cuda):
     rows = q[:1, 0].expand(2**32 + 1, 64)
     with pytest.raises(P, match="2\\^32"):
         pp.sampling.token_logprobs(rows, torch.zeros(1, dtype=torch.int32, device=cuda))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("starts", [[0, 5, 5], [0, 0, 1], [3, 2, 0]])
+def test_starts_are_checked_without_tokens(pp, cuda, starts):
+    """Empty tensors hold no token that starts may name."""
+    N = pp._native
+    bad, none = (torch.tensor(s, dtype=torch.int32, device=cuda) for s in (starts, [0, 0, 0]))
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    empty, keys = torch.empty(0, 2, 64, device=cuda), torch.randn(7, 2, 64, device=cuda)
+    fa = pp.fused_attention
+    ws = fa.prompt_workspace(empty, keys, keys, 2)
+    good = torch.tensor([0, 3, 7], dtype=torch.int32, device=cuda)
+    for k, ks in ((empty, bad), (empty, None), (keys, good)):
+        out = fa.prompt_attention(empty, k, k, bad, kv_starts=ks, status=status.zero_())
+        assert int(status) == N.DEV_LENGTH_RANGE and out.shape == (0, 2, 64)
+    fa.prompt_attention(empty, empty, empty, none, kv_starts=bad, status=status.zero_())
+    assert int(status) == N.DEV_LENGTH_RANGE
+    for k, ks in ((empty, none), (keys, good)):
+        fa.prompt_attention(empty, k, k, none, kv_starts=ks, workspace=ws[:fa.prompt_workspace(empty, k, k, 2).numel()],
+                            status=status.zero_())
+        assert int(status) == 0
+    # the plan of the last call serves one like it
+    fa.prompt_attention(empty, keys, keys, none, kv_starts=good, workspace=ws, plan_ready=True, status=status)
+    assert int(status) == 0
+    arena = pp.kv_cache.Int8KvArena.zeros(2, 2, 64, 16, cuda)
+    arena.append_prompt(empty, empty, bad, none[:2], status=status.zero_())
+    assert int(status) == N.DEV_LENGTH_RANGE
+    arena.append_prompt(empty, empty, bad, none[:2])
+    arena.append_prompt(empty, empty, none, none[:2], status=status.zero_())
+    assert int(status) == 0 and not arena.k.any() and not arena.v_scale.any()
