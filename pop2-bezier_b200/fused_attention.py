@@ -190,9 +190,7 @@ def _prompt_buffers(q: torch.Tensor, workspace: torch.Tensor | None, status: tor
     if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous()
                                   or workspace.device != q.device):
         raise N.PreconditionError("prompt workspace must be a contiguous same-device byte tensor")
-    if status is not None and (status.dtype not in (torch.int32, torch.uint32) or status.numel() < 1
-                               or status.device != q.device):
-        raise N.PreconditionError("prompt status must be a same-device U32 word")
+    ops.check_status(status, q.device)
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts: torch.Tensor, *,

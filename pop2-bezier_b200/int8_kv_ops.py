@@ -63,6 +63,13 @@ def _require_cuda(*ts: torch.Tensor) -> None:
             raise N.PreconditionError("INT8 attention device mismatch")
 
 
+def check_status(status: torch.Tensor | None, device: torch.device) -> None:
+    """A status word is 32 bits that the kernels OR into."""
+    if status is not None and (status.dtype not in (torch.int32, torch.uint32) or status.numel() < 1
+                               or status.device != device):
+        raise N.PreconditionError("status must be a same-device U32 word")
+
+
 def _ptr(t: torch.Tensor | None) -> C.c_void_p:
     return C.c_void_p(t.data_ptr() if t is not None else 0)
 

@@ -143,6 +143,7 @@ class Int8KvArena:
             if t.dtype not in (torch.int32, torch.uint32) or not t.is_contiguous():
                 raise N.PreconditionError("prompt starts and offsets must be contiguous U32")
         N.check_u32(k.shape[0])
+        ops.check_status(status, k.device)
         code = ops._dtype_code(k, "K/V input")
         a = self.struct()
         with ops._here(k):

@@ -80,6 +80,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0,
         raise N.PreconditionError("token logprobs bounds must be contiguous U32 [rows, 2]")
     if not 0 <= top <= 32:
         raise N.PreconditionError("token logprobs give at most 32 alternatives")
+    ops.check_status(status, logits.device)
     code = ops._dtype_code(logits, "logits")
     stride = logits.stride(0) if rows > 1 else choices
     dev = logits.device

@@ -67,3 +67,34 @@ def test_starts_are_checked_without_tokens(pp, cuda, starts):
     arena.append_prompt(empty, empty, bad, none[:2])
     arena.append_prompt(empty, empty, none, none[:2], status=status.zero_())
     assert int(status) == 0 and not arena.k.any() and not arena.v_scale.any()
+
+
+BAD_STATUS = [torch.empty(0, dtype=torch.int32), torch.zeros(1, dtype=torch.uint8), torch.zeros(1, dtype=torch.bfloat16),
+              torch.zeros(1, dtype=torch.int64), torch.zeros(1)]
+
+
+def test_status_words(pp):
+    check, here = pp.int8_kv_ops.check_status, torch.device("cpu")
+    check(None, here), check(torch.zeros(1, dtype=torch.int32), here), check(torch.zeros(3, dtype=torch.uint32), here)
+    for bad in BAD_STATUS:
+        with pytest.raises(pp.PreconditionError, match="status"):
+            check(bad, here)
+    with pytest.raises(pp.PreconditionError, match="status"):
+        check(torch.zeros(1, dtype=torch.int32), torch.device("cuda", 0))
+
+
+@pytest.mark.gpu
+def test_status_words_are_checked(pp, cuda):
+    """The kernels write 32 bits: into a smaller word's neighbours, or nowhere where there is no element."""
+    x = torch.randn(4, 2, 64, device=cuda)
+    starts = torch.tensor([0, 4], dtype=torch.int32, device=cuda)
+    arena = pp.kv_cache.Int8KvArena.zeros(1, 2, 64, 16, cuda)
+    for bad in [b.to(cuda) for b in BAD_STATUS] + [torch.zeros(1, dtype=torch.int32)]:
+        with pytest.raises(pp.PreconditionError):
+            pp.fused_attention.prompt_attention(x, x, x, starts, status=bad)
+        with pytest.raises(pp.PreconditionError):
+            pp.fused_attention.plan_prompt(x, x, x, starts, torch.empty(1 << 20, dtype=torch.uint8, device=cuda), status=bad)
+        with pytest.raises(pp.PreconditionError):
+            arena.append_prompt(x, x, starts, starts[:1], status=bad)
+        with pytest.raises(pp.PreconditionError):
+            pp.sampling.token_logprobs(x[:, 0], starts.repeat(2), status=bad)
