@@ -540,13 +540,13 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prompt_merge_kernel(const __
     // plan_header's check, a word a lane: in registers of every lane it cost a CTA of the three that an SM holds (1023
     // tokens, 24 heads of 64: 25.1 us instead of 22.9).
     const uint32_t word = reinterpret_cast<const uint32_t*>(a.ws)[lane % 8];
+    uint32_t i = blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+    PromptEntry next = load_entry(cuts + min(i / quads / a.kv_heads, a.l.max_ctas - 1));
     const uint32_t n_cuts = __shfl_sync(0xffffffffu, word, 2);
     if (__any_sync(0xffffffffu, lane - 3 < 5 && word != a.key[min(lane - 3, 4u)])) {
         pdl_wait_primary();  // what comes next on the stream waits for this kernel alone
         return;
     }
-    uint32_t i = blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
-    PromptEntry next = load_entry(cuts + min(i / quads / a.kv_heads, a.l.max_ctas - 1));
     pdl_wait_primary();
     while (i < n_cuts * a.kv_heads * quads) {
         const PromptEntry e = next;
