@@ -178,8 +178,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     auto give_up = [&] {
         *abort = 1;
-        // `next` stays where it is, for the list is not handed out to its end: no plan for later calls
-        *reinterpret_cast<volatile uint32_t*>(&reinterpret_cast<PromptHeader*>(a.ws)->key[4]) = 0;
         if (a.status) atomicOr(a.status, PP_DEV_WAIT_TIMEOUT);
     };
     // One thread's wait.
@@ -664,6 +662,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // After giving up `next` stays where it is, for the list is not handed out to its end: no plan for later calls.  (Here
+    // and not in give_up, whose copies stand at every wait: 17 tokens took 9.9 us there and take 9.8, 1023 23.2 and 23.0.)
+    if (threadIdx.x == 0 && *abort) reinterpret_cast<PromptHeader*>(a.ws)->key[4] = 0;
     if (warp == 8) tmem_dealloc(tmem, 512);
 }
 
