@@ -1,5 +1,5 @@
-"""Plans of packed prompts that are kept in a workspace, on the B200: which
-calls one serves, and what the others do."""
+"""Plans of packed prompts on the B200: which calls one that is kept in a workspace
+serves, what the others do, batches of thousands of sequences, two at once."""
 from __future__ import annotations
 
 import pytest
@@ -104,3 +104,46 @@ def test_a_plan_serves_other_strides_and_types(pp, cuda, dtype):
     out = fa.prompt_attention(q, k, v, qs, kv_starts=ks, workspace=ws, plan_ready=True, status=status)
     check(out, q, k, v, [100, 50], [1500, 500], True)
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("sequences", [2047, 2048, 2049, 5000])
+def test_thousands_of_sequences(pp, cuda, sequences):
+    """On both sides of 2048, beyond which the plan keeps the sequences' first entries in the workspace; one of them
+    long, and empty ones throughout and at the end."""
+    lens = [(i * 7919) % 5 for i in range(sequences)]
+    lens[sequences // 3] = 1000
+    lens[-3:] = [0, 0, 0]
+    n = sum(lens)
+    q, k, v = tensors(cuda, n + 2, n + 2, 2, 1, 64, torch.bfloat16, seed=2)
+    out = torch.full_like(q, 7.0)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    starts = starts_of(lens, cuda)
+    pp.fused_attention.prompt_attention(q, k, v, starts, out=out, status=status)
+    assert int(status) == 0 and (out[n:] == 7).all() and out.isfinite().all()
+    at = starts.tolist()
+    for s in sorted({*range(0, sequences, 41), sequences // 3, sequences - 4}):
+        a, b = at[s], at[s + 1]
+        check(out[a:b], q[a:b], k[a:b], v[a:b], [b - a], [b - a], True)
+    bad = starts.clone()
+    bad[-1] = n + 3
+    pp.fused_attention.prompt_attention(q, k, v, bad, out=out.fill_(7), status=status)
+    assert int(status) == pp._native.DEV_LENGTH_RANGE and (out == 7).all()
+
+
+@BOTH
+def test_cut_rows_on_two_streams(pp, cuda, dtype):
+    """Calls whose rows are cut along the keys and merged, on two streams at once."""
+    fa = pp.fused_attention
+    lens, kv = [3, 1, 40], [6000, 3000, 2000]
+    qs, ks = starts_of(lens, cuda), starts_of(kv, cuda)
+    data = [tensors(cuda, 44, 11000, 8, 2, 128, dtype, seed=s) for s in (1, 2)]
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for s in range(2):
+            with torch.cuda.stream(streams[s]):
+                outs[s].append(fa.prompt_attention(*data[s], qs, kv_starts=ks))
+    torch.cuda.synchronize()
+    for s in range(2):
+        check(outs[s][0], *data[s], lens, kv, True)
+        assert all(torch.equal(outs[s][0], o) for o in outs[s])
