@@ -175,8 +175,8 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
 
 // Bounded wait for the phase of `bar` with the given parity.  Gives up when
 // `*abort` is set by another warp or when `limit_ns` elapse, returning false.
-// Every pipeline wait in this library goes through here, so no kernel can
-// spin forever.
+// Every pipeline wait in this library goes through here or through
+// mbar_wait_cycles (tcgen05.cuh), so no kernel can spin forever.
 __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, volatile int* abort,
                                                   uint64_t limit_ns) {
     if (mbar_try_wait(bar, parity)) return true;

@@ -56,7 +56,7 @@ struct Args {
     uint64_t stride;
     const int32_t* targets;
     const uint32_t* bounds;
-    uint32_t rows, choices, top, cluster;
+    uint32_t choices, top, cluster;
     float* logprob;
     float* entropy;
     uint32_t* rank;
@@ -65,7 +65,7 @@ struct Args {
     uint32_t* status;
 };
 
-// What a thread or a CTA knows of a row; the threads of a CTA have one m.
+// What a thread or a CTA knows of a row; the threads of a warp have one m.
 struct Part {
     float m, s, c, d;
     uint32_t ahead;
@@ -613,9 +613,9 @@ __global__ void __launch_bounds__(32 * NW) logprobs_kernel(const Args a) {
 }
 
 template <bool BF, int NW>
-cudaError_t launch(const Args& a, cudaStream_t stream) {
+cudaError_t launch(const Args& a, uint32_t rows, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(a.rows * a.cluster);
+    cfg.gridDim = dim3(rows * a.cluster);
     cfg.blockDim = dim3(32 * NW);
     cfg.dynamicSmemBytes = NW * 32 * kVecs * 16;
     cfg.stream = stream;
@@ -631,12 +631,12 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
 }
 
 template <bool BF>
-cudaError_t launch_warps(const Args& a, uint32_t warps, cudaStream_t stream) {
+cudaError_t launch_warps(const Args& a, uint32_t rows, uint32_t warps, cudaStream_t stream) {
     switch (warps) {
-        case 1: return launch<BF, 1>(a, stream);
-        case 2: return launch<BF, 2>(a, stream);
-        case 4: return launch<BF, 4>(a, stream);
-        default: return launch<BF, kMostWarps>(a, stream);
+        case 1: return launch<BF, 1>(a, rows, stream);
+        case 2: return launch<BF, 2>(a, rows, stream);
+        case 4: return launch<BF, 4>(a, rows, stream);
+        default: return launch<BF, kMostWarps>(a, rows, stream);
     }
 }
 
@@ -648,7 +648,6 @@ cudaError_t launch_token_logprobs(const LogprobsLaunch& L, cudaStream_t stream) 
     a.stride = L.row_stride;
     a.targets = L.targets;
     a.bounds = L.bounds;
-    a.rows = L.rows;
     a.choices = L.choices;
     a.top = L.top;
     a.logprob = L.logprob;
@@ -667,7 +666,7 @@ cudaError_t launch_token_logprobs(const LogprobsLaunch& L, cudaStream_t stream) 
     while (warps < kMostWarps && warps < parts) warps *= 2;
     while (a.cluster < 8 && (uint64_t)L.rows * a.cluster <= L.num_sms && (uint64_t)warps * a.cluster < parts)
         a.cluster *= 2;
-    return L.bf16 ? launch_warps<true>(a, warps, stream) : launch_warps<false>(a, warps, stream);
+    return L.bf16 ? launch_warps<true>(a, L.rows, warps, stream) : launch_warps<false>(a, L.rows, warps, stream);
 }
 
 }  // namespace pp

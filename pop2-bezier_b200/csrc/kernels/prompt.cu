@@ -293,7 +293,6 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 2 : 1) prompt_rows_ker
         if (any) {
             auto token_of = [&](uint32_t r) { return tile_tok + (row0 + r) / a.group; };
             auto live = [&](uint32_t r) { return row0 + r < rows && token_of(r) < e.nq; };
-            // q, scaled so that scores are in log2 units
             for (int i = t; i < 64 * (D / 4); i += kRowsThreads) {
                 const uint32_t r = i / (D / 4), c = i % (D / 4) * 4;
                 float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -658,7 +657,6 @@ PromptArgs prompt_args(const PromptLaunch& L) {
     a.kv_heads = L.g.kv_heads;
     a.group = L.g.heads / L.g.kv_heads;
     a.tpt = kPromptTileRows / a.group;
-    a.q_tokens = L.g.q_tokens;
     a.kv_tokens = L.g.kv_tokens;
     a.causal = L.g.causal;
     a.scale_log2 = L.scale_log2;

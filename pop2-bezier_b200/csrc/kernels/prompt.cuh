@@ -30,7 +30,7 @@ struct PromptArgs {
     PromptWsLayout l;
     uint64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;  // strides in elements
     uint32_t heads, kv_heads, group, tpt;
-    uint32_t q_tokens, kv_tokens;
+    uint32_t kv_tokens;
     uint32_t causal;
     float scale_log2;
     uint32_t vec;  // 16-byte loads of q, k and v rows are aligned
