@@ -13,9 +13,11 @@
  *   k, v  [kv_tokens, kv_heads, head_dim]
  * of `dtype`, head_dim contiguous, with any token and head strides (in
  * elements), so that a view of a QKV projection or of [heads, tokens,
- * head_dim] planes is passed as is.  Query head h reads K/V head
- * h / (heads / kv_heads).  q_tokens and kv_tokens are the rows that the
- * tensors hold; the sequences' own lengths are device data. */
+ * head_dim] planes is passed as is (bf16 on 16-byte boundaries and without
+ * strides of 0 runs on the tensor cores, everything else on the CUDA cores).
+ * Query head h reads K/V head h / (heads / kv_heads).  q_tokens and kv_tokens
+ * are the rows that the tensors hold; the sequences' own lengths are device
+ * data. */
 typedef struct PpPrompt {
     uint32_t struct_size; /* sizeof(PpPrompt) */
     uint32_t sequences;

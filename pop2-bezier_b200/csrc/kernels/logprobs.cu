@@ -26,17 +26,26 @@
 // (on random rows one or two times k of a step's); they wait in a buffer a warp until
 // the row ends; a warp whose buffer is half full keeps its best k.  A candidate's
 // place in the list is the number of candidates ahead of it, which one thread each
-// counts; the order in which they were found does not matter.  Where a step leaves
-// more candidates than the buffer holds (long ties, sorted rows), the block then takes
-// the maximum k times instead: 4096 rows of 32768 in order take 650 us with 5
-// alternatives.  Searching them with a better bound takes 450, but its registers cost
-// random rows 6 to 30 % (81 to 99 us instead of 76).
+// counts; the order in which they were found does not matter.
+//
+// Where a warp finds more candidates in a step than its buffer holds, the block takes
+// the maximum of its part of the row k times instead.  That happens
+//   - where many logits are equal or come in rising order: 4096 rows of 32768, 5
+//     alternatives, 660 us rising and 770 all equal, instead of 76 (searching them with a
+//     better bound took 450, but its registers cost random rows 6 to 30 %);
+//   - where fewer lanes or warps hold logits than the bound counts, so that it stays -inf:
+//     heads and windows of a few times k columns, and the last CTA of a cluster if its
+//     part is short.  4096 rows of 128 bf16: 31 us with 20 alternatives and 43 with 32
+//     instead of 10 with 5; 8 rows of 50257 with 20: 20 us instead of 9 for 65536; 500
+//     columns of 4096 rows of 32768 with 8: 99 us instead of 34 without alternatives.
 //
 // Bound by issue slots and latency: 4096 rows of 32768 bf16 with 5 alternatives 76 us,
-// 3.5 TB/s (maximum and sums alone 51, the rank 8, alternatives 18); 2048 of 131072
-// 121 us, 4.4 TB/s; few rows by latency: 8 of 131072 with 20 alternatives 10 us; 2304
-// windows of up to 1024 f32 8 us.  With a barrier a step 81 and 140 us; with the least
-// of the first ceil(k / q) warps' values as the bound, twice the candidates, 100.
+// 3.5 TB/s, 75 % of issue slots (15.5 warp instructions per 32 logits: 9 for maximum
+// and sums, 2 the rank, 4.5 alternatives; alone they take 51, 8 and 18 us); in f32 142;
+// 2048 of 131072 121 us, 4.4 TB/s; few rows by latency: 8 of 131072 with 20 alternatives
+// 10 us; 2304 windows of up to 1024 f32 8 us.  With a barrier a step 81 and 140 us; with
+// the least of the first ceil(k / q) warps' values as the bound, twice the candidates, 100.
+// In f32 with 8 warps, 8 bytes of spills.
 // Candidates pushed lane by lane, with an atomic each, instead of warp by warp: 98.
 #include <math_constants.h>
 

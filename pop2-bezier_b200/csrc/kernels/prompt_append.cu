@@ -16,8 +16,8 @@
 // RN(m/127) is taken the same way with RN(1/127), by one step, which is right for
 // all 2^23 mantissas (the tests go through them).  Rounding is the addition of
 // 1.5 * 2^23, whose low byte is the code; with |x| <= max|x| no clamp is needed.
-// 16 prompts of 1493 to 2048 tokens, 16 heads of 128: 75 us, 4.7 TB/s, 61 % of issue
-// slots; with the division instruction it took 156.  1023 tokens of 24 heads of 64:
+// 16 prompts of 1493 to 2048 tokens, 16 heads of 128: 73 us, 4.8 TB/s, 61 % of issue
+// slots (f32 97 us, 6.0 TB/s); with the division instruction it took 156.  1023 tokens of 24 heads of 64:
 // 3 us.  Twice the rows a lane, for more loads in flight, cost more registers than
 // they hid.
 // A row that is not finite is divided one by one.  (Dividing only near half

@@ -30,13 +30,17 @@
 // row ends up not finite, and its warp computes it again from the keys that it
 // does see, unless these explain it (prompt.cuh).
 //
-// What bounds it: at head_dim 128 the chain of a tile (S, softmax, P V), of which
-// two run side by side: the softmax of a key tile takes about 1850 cycles and the
-// products with their waits 1400, while the tensor cores need 1024 for both tiles.
-// At 64 the products are half as long and the exponentials bind (16 a clock and SM).
-// 8192 tokens, 16 heads on 4: 1160 TFLOP/s full and 1165 causal at head_dim 128 (71 %
-// of what cuBLAS reaches), 676 and 690 at 64.  Small batches wait for the plan, the
-// first tiles and the code itself: 17 tokens take 10 us, 1023 of 24 heads 24 us.
+// What bounds it: the chain S, softmax, P V of a tile, of which two run side by side.
+// P lies over S, so that S of the next key tile waits until P V has read P, and the
+// softmax waits for both.  Two tiles take 3320 cycles a key tile at head_dim 128, where
+// the tensor cores need 2048 (1024 each) and the exponentials 2048 (2 * 16384, 16 a clock
+// and SM): 62 % of either.  At 64 it is 2930, the tensor cores need 1024 and are busy
+// 35 % of the time, the exponentials 70 %.
+// 8192 tokens, 16 heads on 4: 1165 TFLOP/s full and 1157 causal at head_dim 128 (71 %
+// of what cuBLAS reaches), 671 and 681 at 64; of the full one's time 14 % is the last
+// round, which not all SMs have an item for.  Small batches wait for the plan, the
+// first tiles and the code itself: 17 tokens take 10 us, 1023 of 24 heads 23 us.
+// The softmax's 128 scores a thread cost 32 bytes of spills at head_dim 128.
 // Slower, at the same sizes: P in two halves, so that P V starts earlier (1090: one more
 // wait in the issuing thread at every tile costs more than it hides); that thread
 // waiting for the next K only before its product (1105); one copy of the waits' slow

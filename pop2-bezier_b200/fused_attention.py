@@ -200,13 +200,17 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts
     """Attention of packed prompts; returns [tokens, heads, head_dim] of q's type.
 
     q [tokens, heads, d], k and v [kv_tokens, kv_heads, d], bf16 or f32, any
-    token and head strides; q_starts int32/uint32 [sequences + 1] on the
+    token and head strides (bf16 on 16-byte boundaries and without strides of 0
+    runs on the tensor cores, everything else on the CUDA cores, which takes
+    about ten times as long: pass shared K/V heads as kv_heads, not by expand);
+    q_starts int32/uint32 [sequences + 1] on the
     device: sequence s holds the query tokens q_starts[s] .. q_starts[s + 1].
     kv_starts does the same for the keys (default: the same tokens).  A causal
     query i of n, with m keys, sees keys 0 .. m - n + i: with more keys than
     queries it continues a sequence whose first m - n tokens came before (a
     later chunk of a prompt, or a single token).  A query that sees no key
-    gives NaN; rows of `out` that no sequence holds are left as they were.
+    gives NaN; rows of `out` that no sequence holds are left as they were, and
+    `out` shares no memory with q, k and v.
     softmax_scale 0: 0.125 at d = 64, 1/sqrt(d) otherwise.  A status word gets
     DEV_LENGTH_RANGE when the starts decrease or pass the tensors' ends, and
     DEV_PLAN_MISMATCH when plan_ready finds no plan of this geometry in the
